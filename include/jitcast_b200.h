@@ -194,7 +194,8 @@ jc_status jc_time_attention_device(int device, jc_precision precision, const voi
                                    void* stream);
 
 /* Waits for all work on `device`, then returns and clears the device's kernel error word:
- * JC_ERR_TIMEOUT if a kernel's bounded wait gave up since the last call. */
+ * JC_ERR_TIMEOUT if a kernel's bounded wait gave up since the last call, JC_ERR_INVALID_ARG if a key/value cache
+ * call met device arrays outside its bounds. */
 jc_status jc_device_sync(int device);
 
 /* ===================================================================================== */
@@ -484,6 +485,108 @@ jc_status jc_timestral_finish_device(int device, int rows, int steps, int quanti
 jc_status jc_chronos2_finish_device(int device, int rows, int output_patches, int patch, int quantiles,
                                     int use_arcsinh, const float* loc_scale, const float* raw, float* out,
                                     void* stream);
+
+/* ===================================================================================== */
+/* A paged key/value cache: keys and values kept between calls, and attention over them.   */
+/* ===================================================================================== */
+
+/*
+ * No counterpart in the reference, whose forwards recompute a series' whole context each time
+ * (timestral/tornado/TimestralForward.java:187-642): for callers that keep a layer's keys and values while
+ * patches arrive. The three calls below work on one layer's cache and may be captured into CUDA graphs. A call's
+ * device arrays are read when its kernels run, on `stream`.
+ *
+ * The pools (device memory, 16-byte aligned), contiguous, head_dim D 64 or 128, page_size a multiple of 16:
+ *   bits 16: k, v [pages, kv_heads, page_size, D] in the call's precision (JC_BF16 or JC_FP16)
+ *   bits 4:  k, v [pages, kv_heads, page_size, D / 2] bytes: byte j holds dim 2j in its low half and 2j + 1 in its
+ *            high half; k_scale, v_scale [pages, kv_heads, page_size, D / 32] FP16 pairs (scale, min), one per 32
+ *            consecutive dims: code c stands for fp16(c * scale + min). The tensors around the cache are in the
+ *            call's precision.
+ */
+typedef struct jc_kv_cache {
+  int bits;
+  int pages;
+  int page_size;
+  int kv_heads;
+  int head_dim;
+  void* k;
+  void* v;
+  void* k_scale; /* bits 4 only */
+  void* v_scale;
+} jc_kv_cache;
+
+/*
+ * The sequences of a call. Sequence s has `length[s]` cached tokens, its n new ones of this step among them
+ * (n = start[s + 1] - start[s], their packed rows in order), so new token i has index length[s] - n + i; index t
+ * lives in slot t % page_size of page page_table[s][t / page_size]. A new token whose index would be below 0 is
+ * not stored and sees no key. `start` NULL: one new token per sequence, row s (tokens = sequences, max_new = 1).
+ *
+ * max_new and max_length bound every sequence (they shape the launch). The arrays live on the device: a sequence
+ * whose start, length or page ids lie outside the call's bounds (pages: [0, cache pages)) is left out (an attention
+ * row leaves out the page's keys), no memory outside the given arrays is touched, and the next jc_device_sync
+ * returns JC_ERR_INVALID_ARG. Page ids past a sequence's length, and in pages that its tokens do not see, are not
+ * read. No two sequences of an append may own one page that it writes.
+ */
+typedef struct jc_kv_step {
+  int sequences;
+  int tokens;     /* packed rows of the tensors of new tokens */
+  int max_new;    /* most new tokens of one sequence */
+  int max_length; /* most cached tokens of one sequence */
+  const int32_t* start;      /* [sequences + 1] or NULL */
+  const int32_t* length;     /* [sequences] */
+  const int32_t* page_table; /* [sequences, table_pages], row pitch ld_table */
+  int table_pages;
+  long long ld_table;
+} jc_kv_step;
+
+/* Rows of heads on the device in the call's precision: element (row, head, dim) at row * ld + head * head_stride +
+ * dim elements (a column block of a q|k|v product is such a tensor). Any strides; 16-byte aligned ones are faster. */
+typedef struct jc_kv_rows {
+  void* data;
+  long long ld;
+  long long head_stride;
+} jc_kv_rows;
+
+/*
+ * Appends the step's new keys and values to the cache, keys and queries rotated on the way (RoPE):
+ *   k, v [tokens, kv_heads, D]; q [tokens, heads, D] and q_out of the same shape (both NULL: no queries; q_out may
+ *   be q itself). rope_table [rope_rows, D] FP32: the cosine of pair e at e, its sine at D / 2 + e; the pairs
+ *   (e, e + D / 2) with e < rope_pairs rotate by row positions[token] (positions NULL: the token's index), as the
+ *   engines' fused RoPE does. rope_table NULL: nothing rotates.
+ * Rotated in FP32, each product and sum rounded once, then stored in the precision (FP16 saturating) or in 4 bits:
+ * scale = fp16((max - min) / 15) and min = fp16(min) of the 32 FP32 values (saturated at +-65504; the scale a little
+ * smaller where the top code would pass FP16's range), codes the nearest of the 16 steps. A group with a NaN reads
+ * back as NaN.
+ */
+jc_status jc_kv_append_device(int device, jc_precision precision, const jc_kv_cache* cache, const jc_kv_step* step,
+                              const jc_kv_rows* k, const jc_kv_rows* v, const jc_kv_rows* q, int heads,
+                              const jc_kv_rows* q_out, const int32_t* positions, const float* rope_table,
+                              int rope_rows, int rope_pairs, void* stream);
+
+/*
+ * Attention of the step's new tokens over the cache (which holds them already): with index t, a token sees the keys
+ * j <= t with j > t - window or j < sinks (window 0: every j <= t);
+ *   out [tokens, heads, D] = sum_j softmax_j(scale * q.k_j) v_j, zeros for a token that sees no key.
+ * Query head h reads kv head h / (heads / kv_heads). Statistics and sums are held in FP32. Values in slots that a
+ * token does not see never reach its output, whatever they are. `workspace` (16-byte aligned device memory, NULL
+ * when jc_kv_attention_workspace says 0) holds partial results during the call; its contents do not matter.
+ */
+jc_status jc_kv_attention_device(int device, jc_precision precision, const jc_kv_cache* cache, const jc_kv_step* step,
+                                 const jc_kv_rows* q, int heads, const jc_kv_rows* out, int window, int sinks,
+                                 float scale, void* workspace, long long workspace_bytes, void* stream);
+
+/* Bytes of workspace that jc_kv_attention_device needs for these arguments (host arithmetic only; no pointer of
+ * `cache` or `step` is read through). */
+jc_status jc_kv_attention_workspace(jc_precision precision, const jc_kv_cache* cache, const jc_kv_step* step,
+                                    int heads, int window, int sinks, long long* bytes);
+
+/*
+ * Reads the step's new tokens (give n = length to read whole sequences) back from the cache into k, v
+ * [tokens, kv_heads, D]: the precision's values of a 16-bit cache, FP16 values of a 4-bit one whatever the
+ * precision. Zeros for a token of index below 0.
+ */
+jc_status jc_kv_read_device(int device, jc_precision precision, const jc_kv_cache* cache, const jc_kv_step* step,
+                            const jc_kv_rows* k, const jc_kv_rows* v, void* stream);
 
 /*
  * Self-test of the bounded waits every kernel of the library uses (no counterpart in the reference): one

@@ -6,7 +6,7 @@ interfaces over that ABI: ``ops`` (Kernels.gemm / Ops.linear) and one module per
 """
 
 from ._lib import BF16, FP32, TF32, JcArgumentError, JcError, JcUnavailable, lib  # noqa: F401
-from . import ops  # noqa: F401
+from . import kvcache, ops  # noqa: F401
 
 __version__ = "0.1.0"
 

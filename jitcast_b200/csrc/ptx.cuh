@@ -25,6 +25,7 @@ enum DeviceError : uint32_t {
   kErrAttnWait = 1u << 5,      // the attention kernel waited too long for a TMA load or an MMA
   kErrTimeoutPeer = 1u << 6,   // a recurrent cell waited too long for its cluster peers' state
   kErrTimeoutResidual = 1u << 7,  // a GEMM epilogue waited too long for its staged residual tile
+  kErrKvStep = 1u << 8,        // a cache step's starts, lengths, pages or positions lie outside the call's bounds
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -91,6 +91,8 @@ jc_status take_device_error(DeviceRt* rt) {
   if (host) {
     cudaMemsetAsync(rt->err, 0, sizeof(uint32_t), rt->stream);
     cudaStreamSynchronize(rt->stream);
+    if (host == kErrKvStep)
+      return fail(JC_ERR_INVALID_ARG, "a cache step's starts, lengths, pages or positions lie outside its call's bounds");
     return fail(JC_ERR_TIMEOUT, "a device wait gave up (error bits 0x" + [&] {
       char b[16];
       snprintf(b, sizeof b, "%x", host);
