@@ -1,0 +1,94 @@
+// What the cache attention's kernels share: which keys a token sees, the ranges of 16-key blocks that a tile of
+// query rows reads, and the row-by-row form that recomputes a row whose result is not a number.
+#pragma once
+
+#include "kvcache.cuh"
+
+namespace jc {
+
+// The keys that index t sees are [0, sink) and [first, t + 1).
+__device__ __forceinline__ int kv_first(const KvAttnArgs& a, int t) {
+  return a.window > 0 && t + 1 > a.window ? t + 1 - a.window : 0;
+}
+
+// The 16-key blocks that the tokens t0 .. t1 of one sequence read: blocks 0 .. a − 1 (sinks), then b .. b + n − a − 1;
+// n in all, none twice. A page holds a whole number of blocks.
+struct KvBlocks {
+  int a, b, n;
+  __device__ __forceinline__ int at(int x) const { return x < a ? x : x - a + b; }
+};
+
+__device__ __forceinline__ KvBlocks kv_blocks(const KvAttnArgs& a, int t0, int t1) {
+  KvBlocks k;
+  if (t1 < 0) return KvBlocks{0, 0, 0};
+  k.b = kv_first(a, t0 < 0 ? 0 : t0) >> 4;
+  const int sink = a.sinks < t1 + 1 ? a.sinks : t1 + 1;
+  k.a = (sink + 15) >> 4;
+  if (k.a > k.b) k.a = k.b;
+  k.n = k.a + (t1 >> 4) - k.b + 1;
+  return k;
+}
+
+// One row of the output by one warp, key by key on the CUDA cores in FP32 (lane l holds dims l, l + 32, ..),
+// with the running maximum and sum of the softmax. It reads visible keys alone. The tiled kernels multiply a hidden
+// key's value by a probability of 0, which is NaN for an infinite or undefined value; they hand a row that comes
+// out with a NaN to this form, so hidden values stay out of every result and a visible NaN stays in it.
+template <typename T, int BITS, int D>
+__device__ __noinline__ void kv_attend_row(const KvAttnArgs& a, int s, int t, int head, const T* q, T* out) {
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int kvh = head / (a.heads / a.c.kv_heads);
+  const int* table = a.st.table + s * a.st.ld_table;
+  float x[N], o[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    x[i] = kv_float(q[lane + 32 * i]) * a.scale;
+    o[i] = 0.0f;
+  }
+  float m = -INFINITY, l = 0.0f;
+  const int first = kv_first(a, t), sink = a.sinks < first ? a.sinks : first;
+  for (int j = sink > 0 ? 0 : first; j <= t; j = j + 1 == sink ? first : j + 1) {
+    const long long page = kv_page_row(a.c, table, j / a.c.page_size, kvh);
+    if (page < 0) {
+      if (lane == 0) atomicOr(a.err, kErrKvStep);
+      continue;
+    }
+    const long long row = page + j % a.c.page_size;
+    float d = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) d = fmaf(x[i], kv_value<T, BITS>(a.c.k, a.c.k_scale, row, D, lane + 32 * i), d);
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
+    const float mn = fmaxf(m, d);
+    const float up = mn == -INFINITY ? 1.0f : __expf(m - mn);  // −inf − −inf would be NaN
+    const float p = mn == -INFINITY ? 0.0f : d != d ? d : __expf(d - mn);
+    l = l * up + p;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = o[i] * up + p * kv_value<T, BITS>(a.c.v, a.c.v_scale, row, D, lane + 32 * i);
+    m = mn;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[lane + 32 * i] = kv_round<T>(o[i] * inv);
+}
+
+// 2^x by the special-function unit: 2 ulp, flushes subnormal results (a probability below 2^-126 is none).
+__device__ __forceinline__ float kv_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Division of 0 <= u < 2^27 (a 16-key block of a 31-bit length) by a page's blocks, as a product: m = 2^32 / d
+// rounded up is off by less than one in d · m, so u · m / 2^32 is exact while u · d < 2^32 (d <= 32, pages of up to 512
+// tokens) and larger pages divide.
+struct KvDiv {
+  unsigned d;
+  unsigned long long m;
+  __host__ __device__ KvDiv(unsigned by = 1) : d(by), m((1ull << 32) / by + ((1ull << 32) % by ? 1 : 0)) {}
+  __device__ __forceinline__ unsigned of(unsigned u) const {
+    return d <= 32 ? static_cast<unsigned>((u * m) >> 32) : u / d;
+  }
+};
+
+}  // namespace jc
