@@ -633,7 +633,7 @@ cudaError_t attend(const KvAttnArgs& a, cudaStream_t s) {
 }  // namespace
 
 long long kv_attention_workspace(const KvAttnArgs& a) {
-  if (a.st.sequences == 0 || a.st.max_new == 0) return 0;
+  if (a.st.sequences == 0 || a.st.max_new == 0 || kv_attention_tc_ok(a)) return 0;
   const SplitShape sh = shape_of(a);
   if (sh.splits == 1) return 0;
   return static_cast<long long>(sh.splits) * a.st.tokens * a.heads * (a.c.dim + 2) * 4;
@@ -641,6 +641,7 @@ long long kv_attention_workspace(const KvAttnArgs& a) {
 
 cudaError_t launch_kv_attention(const KvAttnArgs& a, cudaStream_t s) {
   if (a.st.sequences == 0 || a.st.max_new == 0) return cudaSuccess;
+  if (kv_attention_tc_ok(a)) return launch_kv_attention_tc(a, s);
   if (a.c.bits == 16) {
     if (a.c.dim == 64)
       return a.c.f16 ? attend<__half, 16, 64>(a, s) : attend<__nv_bfloat16, 16, 64>(a, s);

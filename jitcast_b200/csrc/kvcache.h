@@ -76,6 +76,10 @@ cudaError_t launch_kv_append(const KvAppendArgs& a, cudaStream_t s);
 cudaError_t launch_kv_read(const KvReadArgs& a, cudaStream_t s);
 cudaError_t launch_kv_attention(const KvAttnArgs& a, cudaStream_t s);
 
+// The form on 128-row tcgen05 tiles (kv_attention_tc.cu), for the calls that take it.
+bool kv_attention_tc_ok(const KvAttnArgs& a);
+cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, cudaStream_t s);
+
 // Bytes of workspace that launch_kv_attention needs for this call (0: none); reads no pointer.
 long long kv_attention_workspace(const KvAttnArgs& a);
 
