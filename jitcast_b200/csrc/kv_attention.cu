@@ -213,7 +213,7 @@ __device__ __forceinline__ Tile tile_of(const KvAttnArgs& a, const KvSeq& q, int
   x.rows = min(q.n * group - r0, most);
   x.t0 = q.length - q.n + r0 / group;
   x.t1 = q.length - q.n + (r0 + x.rows - 1) / group;
-  x.kb = x.rows > 0 ? kv_blocks(a, x.t0, x.t1) : KvBlocks{0, 0, 0};
+  x.kb = x.rows > 0 ? kv_blocks(a, x.t0, x.t1, 4) : KvBlocks{0, 0, 0};
   return x;
 }
 
@@ -236,7 +236,8 @@ __device__ __forceinline__ void store4(T* p, float4 v, bool vec) {
 }
 
 template <typename T, int BITS, int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(const KvAttnArgs a, const SplitShape sh) {
+__global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(const __grid_constant__ KvAttnArgs a,
+                                                                      const __grid_constant__ SplitShape sh) {
   using F = Frag<BITS, D>;
   using M = std::conditional_t<BITS == 4, __half, T>;  // the products' type
   constexpr int ROWS = 8 * NT, SUB = F::SUB, PITCH = D + 4;
@@ -518,7 +519,8 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(const K
 // Joins the splits of each output row: D / 4 lanes a row, the splits in order. HBM / L2 bound: it reads what the
 // splits wrote once; launched early (programmatic dependent launch), it waits for them on the device.
 template <typename T, int BITS, int D>
-__global__ void __launch_bounds__(128) kv_combine_kernel(const KvAttnArgs a, const SplitShape sh, int rows_per_tile) {
+__global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__ KvAttnArgs a,
+                                                         const __grid_constant__ SplitShape sh, int rows_per_tile) {
   constexpr int LANES = D / 4;
   const int lane = threadIdx.x & 31;
   const int seq = blockIdx.y;

@@ -11,21 +11,21 @@ __device__ __forceinline__ int kv_first(const KvAttnArgs& a, int t) {
   return a.window > 0 && t + 1 > a.window ? t + 1 - a.window : 0;
 }
 
-// The 16-key blocks that the tokens t0 .. t1 of one sequence read: blocks 0 .. a − 1 (sinks), then b .. b + n − a − 1;
-// n in all, none twice. A page holds a whole number of blocks.
+// The blocks of 2^shift keys that the tokens t0 .. t1 of one sequence read: blocks 0 .. a − 1 (sinks), then
+// b .. b + n − a − 1; n in all, none twice. A page holds a whole number of blocks.
 struct KvBlocks {
   int a, b, n;
   __device__ __forceinline__ int at(int x) const { return x < a ? x : x - a + b; }
 };
 
-__device__ __forceinline__ KvBlocks kv_blocks(const KvAttnArgs& a, int t0, int t1) {
+__device__ __forceinline__ KvBlocks kv_blocks(const KvAttnArgs& a, int t0, int t1, int shift) {
   KvBlocks k;
   if (t1 < 0) return KvBlocks{0, 0, 0};
-  k.b = kv_first(a, t0 < 0 ? 0 : t0) >> 4;
+  k.b = kv_first(a, t0 < 0 ? 0 : t0) >> shift;
   const int sink = a.sinks < t1 + 1 ? a.sinks : t1 + 1;
-  k.a = (sink + 15) >> 4;
+  k.a = (sink >> shift) + ((sink & ((1 << shift) - 1)) != 0 ? 1 : 0);
   if (k.a > k.b) k.a = k.b;
-  k.n = k.a + (t1 >> 4) - k.b + 1;
+  k.n = k.a + (t1 >> shift) - k.b + 1;
   return k;
 }
 

@@ -46,10 +46,11 @@ struct TcCfg {
 };
 
 struct TcArgs {
+  int shift;         // 2^shift keys a block: the largest power of two, up to 64, that a page holds a whole number of
   int supers;        // 256-row tiles of the longest sequence
   int pool_rows;     // rows of the pools: a coordinate outside them
   int vec_q, vec_o;  // 16-byte vectors
-  KvDiv page;
+  KvDiv page;        // blocks of a page
 };
 
 __device__ __forceinline__ uint32_t sw128(int r, int c) {
@@ -65,6 +66,28 @@ __device__ __forceinline__ uint32_t pack_p(float a, float b) {
     __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
   }
+}
+
+// Two FP32 values in one 64-bit register: one instruction adds or multiplies both.
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 // Bits lo .. hi − 1 of 16.
@@ -93,7 +116,8 @@ __device__ __forceinline__ uint64_t sdesc_v(uint32_t saddr, uint32_t atom_bytes)
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK,
                                                                        const __grid_constant__ CUtensorMap tmV,
-                                                                       const KvAttnArgs a, const TcArgs tc) {
+                                                                       const __grid_constant__ KvAttnArgs a,
+                                                                       const __grid_constant__ TcArgs tc) {
   using C = TcCfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -124,8 +148,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
   if (rows <= 0) return;
   const int base_t = sq.length - sq.n;
   const int t0 = base_t + r0 / group, t1 = base_t + (r0 + rows - 1) / group;
-  const KvBlocks kb = kv_blocks(a, t0, t1);
-  const int steps = (kb.n + 7) >> 3;
+  const KvBlocks kb = kv_blocks(a, t0, t1, tc.shift);
+  const int per = kKeys >> tc.shift;  // blocks of a step
+  const int steps = (kb.n + per - 1) >> (7 - tc.shift);
   const int tiles = rows > kRows ? 2 : 1;
   const int* table = a.st.table + seq * a.st.ld_table;
 
@@ -167,59 +192,63 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
   if (good && warp >= 8) {
    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcRegsIssue));
    if (warp == 8) {
-    // ---- producer: lane = 16-key block (and 64-dim column block) of a step ----
-    constexpr int LANES = 8 * (D / 64);
-    const int blk = lane & 7, atom = lane >> 3;
-    const int first = kv_first(a, t0 < 0 ? 0 : t0);
+    // ---- producer: lane = block (and 64-dim column block) of a step ----
+    const int blk = lane & (per - 1), atom = lane >> (7 - tc.shift);
+    const bool mine = atom < D / 64;
+    const int size = 1 << tc.shift, first = kv_first(a, t0 < 0 ? 0 : t0);
+    const uint32_t off = atom * C::ATOM + blk * (size * 128);
     bool ok = true;
     uint32_t raw_phase = 0;
+    // the pool row of the lane's block in step j; past the last block: outside the pool, which loads zeros
+    auto row_of = [&](int j) -> int {
+      const int x = j * per + blk;
+      if (!mine || x >= kb.n) return tc.pool_rows;
+      const int b = kb.at(x);
+      const unsigned pg = tc.page.of(b);
+      return (__ldg(table + pg) * a.c.kv_heads + kvh) * a.c.page_size + ((b - static_cast<int>(pg * tc.page.d)) << tc.shift);
+    };
+    int row = row_of(0);
     for (int j = 0; j < steps && ok; ++j) {
       const int st = j % C::STAGES;
       const uint32_t ph = (j / C::STAGES) & 1;
-      const int x = 8 * j + blk;
-      const int b = kb.at(x);
-      int row = tc.pool_rows;  // past the last block: outside the pool, which loads zeros
-      if (x < kb.n) {
-        const unsigned pg = tc.page.of(b);
-        row = (__ldg(table + pg) * a.c.kv_heads + kvh) * a.c.page_size +
-              ((b - static_cast<int>(pg * tc.page.d)) << 4);
-      }
+      const int next = row_of(j + 1);  // in flight during this step's waits
       if (!mbar_wait(k_free + st, ph ^ 1) || *abort_flag) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (lane == 0) mbar_arrive_expect_tx(k_full + st, C::TILE);
       __syncwarp();
-      if (lane < LANES)
-        tma_load_2d(smem + C::K_OFF + st * C::TILE + atom * C::ATOM + blk * 2048, &tmK, k_full + st, 64 * atom, row);
+      if (mine) tma_load_2d(smem + C::K_OFF + st * C::TILE + off, &tmK, k_full + st, 64 * atom, row);
       if (!mbar_wait(v_free + st, ph ^ 1) || *abort_flag) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      // keys of the block that no row of the CTA sees: their values, whatever they are, become zeros
-      uint32_t seen = 0u;
-      if (x < kb.n) seen = bits16(0, t1 + 1 - (b << 4)) & (bits16(first - (b << 4), 16) | bits16(0, a.sinks - (b << 4) > 16 ? 16 : a.sinks - (b << 4)));
-      const bool clear = __any_sync(0xffffffffu, x < kb.n && seen != 0xFFFFu);
-      uint8_t* vt = smem + C::V_OFF + st * C::TILE;
+      // keys of the step that no row of the CTA sees: their values, whatever they are, become zeros
+      const int x = j * per + blk, key0 = kb.at(x) << tc.shift;
+      const bool part = mine && x < kb.n && (key0 + size - 1 > t1 || (key0 < first && key0 + size > a.sinks));
+      const bool clear = __any_sync(0xffffffffu, part);
+      uint8_t* vt = smem + C::V_OFF + st * C::TILE + off;
       uint64_t* bar = clear ? v_raw : v_full + st;
       if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
       __syncwarp();
-      if (lane < LANES) tma_load_2d(vt + atom * C::ATOM + blk * 2048, &tmV, bar, 64 * atom, row);
+      if (mine) tma_load_2d(vt, &tmV, bar, 64 * atom, row);
       if (clear) {
         ok = mbar_wait(v_raw, raw_phase);
         raw_phase ^= 1;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (lane < LANES && x < kb.n) {
-          for (int r = 0; r < 16; ++r)
-            if (!((seen >> r) & 1u)) {
-              uint4* p = reinterpret_cast<uint4*>(vt + atom * C::ATOM + blk * 2048 + r * 128);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) p[i] = make_uint4(0u, 0u, 0u, 0u);
-            }
+        for (uint32_t left = __ballot_sync(0xffffffffu, part); left; left &= left - 1) {
+          const int from = __ffs(left) - 1;  // the whole warp clears that lane's block
+          const int k0 = __shfl_sync(0xffffffffu, key0, from);
+          uint8_t* p = smem + C::V_OFF + st * C::TILE + __shfl_sync(0xffffffffu, off, from);
+          for (int w = lane; w < size * 8; w += 32) {
+            const int key = k0 + (w >> 3);
+            if (key > t1 || (key < first && key >= a.sinks)) *reinterpret_cast<uint4*>(p + 16 * w) = make_uint4(0u, 0u, 0u, 0u);
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(v_full + st);
       }
+      row = next;
     }
     if (!ok) {
       if (lane == 0) {
@@ -342,28 +371,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_col + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s[c]));
           tmem_ld_wait();
-          float mx = -INFINITY;
+          // Hide what a row does not see. A step of the band that every row of the warp sees whole skips this.
+          const int key0 = kb.at(j * per) << tc.shift;
+          if (!(j * per >= kb.a && key0 + kKeys - 1 <= tw0 && key0 >= fw1)) {
+            const int sub = tc.shift - 4;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int ka = kb.at(8 * j + 2 * c) << 4, kc = kb.at(8 * j + 2 * c + 1) << 4;
-            const bool open = (ka + 15 <= tw0 && (ka >= fw1 || ka + 16 <= a.sinks)) &&
-                              (kc + 15 <= tw0 && (kc >= fw1 || kc + 16 <= a.sinks));
-            const bool closed = (ka > tw1 || (ka + 15 < fw0 && ka >= a.sinks)) &&
-                                (kc > tw1 || (kc + 15 < fw0 && kc >= a.sinks));
-            if (closed) {
-              shut |= 1u << c;
-            } else {
-              if (!open) {
-                const uint32_t bits = block_bits(ka, t, first, a.sinks) | block_bits(kc, t, first, a.sinks) << 16;
+            for (int c = 0; c < 4; ++c) {
+              const int ha = 8 * j + 2 * c, hc = ha + 1;  // the chunk's two 16-key halves
+              const int ka = (kb.at(ha >> sub) << tc.shift) + ((ha & ((1 << sub) - 1)) << 4);
+              const int kc = (kb.at(hc >> sub) << tc.shift) + ((hc & ((1 << sub) - 1)) << 4);
+              if ((ka > tw1 || (ka + 15 < fw0 && ka >= a.sinks)) && (kc > tw1 || (kc + 15 < fw0 && kc >= a.sinks))) shut |= 1u << c;
+              const uint32_t bits = block_bits(ka, t, first, a.sinks) | block_bits(kc, t, first, a.sinks) << 16;
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (!((bits >> e) & 1u)) s[c][e] = -INFINITY;
-              }
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) mx = fmax3(mx, s[c][e], s[c][e + 1]);
+              for (int e = 0; e < 32; ++e)
+                if (!((bits >> e) & 1u)) s[c][e] = -INFINITY;
             }
           }
-          const float top = mx * sl2;
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) mx4[(e >> 1) & 3] = fmax3(mx4[(e >> 1) & 3], s[c][e], s[c][e + 1]);
+          const float top = fmax3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * sl2;
           if (__any_sync(0xffffffffu, top > m + kTcLazy)) {
             const float mn = fmaxf(m, top);
             const float up = mn == -INFINITY ? 1.0f : kv_ex2(m - mn);
@@ -382,6 +411,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
             }
           }
           const float base = m == -INFINITY ? 0.0f : m;
+          uint64_t l2[4] = {0ull, 0ull, 0ull, 0ull};  // pairs of partial row sums
+          const uint64_t sc2 = pack_f32x2(sl2, sl2), base2 = pack_f32x2(-base, -base);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t pk[16];
@@ -391,13 +422,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
             } else {
 #pragma unroll
               for (int e = 0; e < 32; e += 2) {
-                const float p0 = kv_ex2(fmaf(s[c][e], sl2, -base)), p1 = kv_ex2(fmaf(s[c][e + 1], sl2, -base));
-                l += p0 + p1;
+                const float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(s[c][e], s[c][e + 1]), sc2, base2));
+                const float p0 = kv_ex2(x.x), p1 = kv_ex2(x.y);
+                l2[(e >> 1) & 3] = add_f32x2(l2[(e >> 1) & 3], pack_f32x2(p0, p1));
                 pk[e >> 1] = pack_p<T>(p0, p1);
               }
             }
             tmem_st_32x32b_x16(s_col + 16 * c, pk);
           }
+          const float2 la = unpack_f32x2(add_f32x2(add_f32x2(l2[0], l2[1]), add_f32x2(l2[2], l2[3])));
+          l += la.x + la.y;
           tmem_st_wait();
         }
         tc_fence_before();
@@ -484,10 +518,12 @@ cudaError_t launch_tc(const KvAttnArgs& a, cudaStream_t s) {
   };
   tc.vec_q = fits(a.q);
   tc.vec_o = fits(a.out);
-  tc.page = KvDiv(static_cast<unsigned>(a.c.page_size / 16));
+  tc.shift = a.c.page_size % 64 == 0 ? 6 : a.c.page_size % 32 == 0 ? 5 : 4;
+  tc.page = KvDiv(static_cast<unsigned>(a.c.page_size >> tc.shift));
   CUtensorMap mk, mv;
   const int op = std::is_same<T, __half>::value ? kOpF16 : kOpBF16;
-  if (!make_operand_map(&mk, a.c.k, op, tc.pool_rows, D, D, 16) || !make_operand_map(&mv, a.c.v, op, tc.pool_rows, D, D, 16))
+  if (!make_operand_map(&mk, a.c.k, op, tc.pool_rows, D, D, 1 << tc.shift) ||
+      !make_operand_map(&mv, a.c.v, op, tc.pool_rows, D, D, 1 << tc.shift))
     return cudaErrorInvalidValue;
   cudaError_t e = cudaFuncSetAttribute(kv_attention_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return e;

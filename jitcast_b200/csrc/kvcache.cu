@@ -99,7 +99,7 @@ __device__ __forceinline__ uint32_t quantise8(float (&x)[8], __half2& sm) {
 }
 
 template <typename T, int BITS, int D, bool VEC>
-__global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs a) {
+__global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ KvAppendArgs a) {
   constexpr int TPH = D / 16;  // threads per head
   const int row = blockIdx.x;
   const int s = kv_seq_of(a.st, row);
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs a) {
 
 // Cached tokens as packed rows of 16-bit values (a 4-bit cache: FP16, the values its codes stand for).
 template <typename T, int BITS, int D, bool VEC>
-__global__ void __launch_bounds__(256) kv_read_kernel(const KvReadArgs a) {
+__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvReadArgs a) {
   constexpr int TPH = D / 8;
   const int row = blockIdx.x;
   const int s = kv_seq_of(a.st, row);
