@@ -6,15 +6,17 @@
 //   S_i = Q_i · Kᵀ    tcgen05.mma kind::f16, Q and K K-major in shared memory, S in TMEM (128 × 128 FP32)
 //   O_i += P_i · V    P from TMEM (over S's columns, 16 bits), V MN-major in shared memory, O in TMEM
 //
-// Four softmax warps a tile (a thread a row: running maximum and sum need no shuffle), one TMA producer
-// warp (a lane a 16-key block: pages may lie anywhere) and one MMA issuer. The two tiles alternate: while one tile's
-// products run, the other's exponentials do, and both read each K and V tile once from shared memory, which halves
-// the bytes from L2. What bounds it: at 64 dims the exponentials (128 · 128 a tile at 16 a clock and SM: 1024 clocks,
-// against 512 for the products), at 128 dims both alike.
+// Four softmax warps a tile (a thread a row: running maximum and sum need no shuffle), one TMA producer warp (a lane
+// a block of keys: pages may lie anywhere) and one MMA issuer. The two tiles alternate: while one tile's products run,
+// the other's exponentials do, and both read each K and V tile once from shared memory, which halves the bytes from L2.
+// What bounds it: at 64 dims the exponentials (128 · 128 a tile at 16 a clock and SM: 1024 clocks, against 512 for the
+// products), at 128 dims both alike; a step takes 1.5 to 1.9 times that, the latencies of the chain product → TMEM load
+// → exponentials → TMEM store → product that the other tile (or CTA) does not cover. Taking some exponentials on the FMA
+// units by a polynomial made it slower (issue slots), P in TMEM columns of its own too (one more handshake a step).
 //
-// The running maximum moves only when a score passes it by 2^kLazy (as in the split kernel), so O is rescaled in
-// TMEM in few steps. S(j + 1) is issued after P·V(j) of its tile by the same thread, so when a softmax warp sees
-// S(j + 1) ready, O holds every P·V up to j and no product is touching it.
+// S(j + 1) is issued after P·V(j) of its tile by the same thread, so when a softmax warp sees S(j + 1) ready, O holds
+// every P·V up to j and no product is touching it: the rare rescaling of O (where the running maximum moves by much)
+// needs no barrier of its own.
 #include <algorithm>
 
 #include "gemm.h"
@@ -25,24 +27,34 @@ namespace jc {
 namespace {
 
 constexpr int kRows = 128;   // rows of a tile (TMEM lanes)
-constexpr int kKeys = 128;   // keys of a step
-constexpr int kTcThreads = 384;
-// Registers a thread: 168 at launch (three warps on each SM quarter); the third warpgroup gives some of its to the
-// softmax warpgroups, which hold a row of 128 scores. 2 · 224 + 56 = 3 · 168.
-constexpr int kTcRegs = 168, kTcRegsSoftmax = 224, kTcRegsIssue = 56;
 constexpr float kTcLog2e = 1.4426950408889634f;
 constexpr float kTcLazy = 8.0f;
 
-template <int D>
+// LONG 0 (64 dims): 64 keys a step, so that S and O of both tiles take 256 TMEM columns and two CTAs fit on an SM: a
+// CTA's start and end run under the other's steps.
+// LONG 1: 128 keys a step and one CTA an SM; its softmax warps hold their rows' 128 scores, for which the third
+// warpgroup gives up registers (168 a thread at launch: 2 · 208 + 88 = 3 · 168).
+template <int D, int LONG>
 struct TcCfg {
-  static constexpr int STAGES = D == 64 ? 4 : 2;
-  static constexpr int TILE = kKeys * D * 2;    // bytes of a K, V or Q tile
+  static_assert(LONG || D == 64, "the short form is for 64 dims");
+  static constexpr int KEYS = LONG ? 128 : 64;     // keys of a step
+  static constexpr int LOG_KEYS = LONG ? 7 : 6;
+  static constexpr int CTAS = LONG ? 1 : 2;        // on an SM
+  static constexpr int THREADS = LONG ? 384 : 320;
+  static constexpr bool SPLIT_REGS = LONG, HOLD = LONG;
+  static constexpr int REGS = 168, REGS_SOFTMAX = 208, REGS_ISSUE = 88;
+  static constexpr int STAGES = LONG && D == 128 ? 2 : 4;
+  static constexpr int Q_TILE = kRows * D * 2;     // bytes of a Q (and at the end an output) tile
+  static constexpr int TILE = KEYS * D * 2;        // bytes of a K or V tile
+  static constexpr int ATOM = KEYS * 128;          // of its 64-dim column blocks (128-byte swizzled rows)
+  static constexpr int Q_ATOM = kRows * 128;
   static constexpr int Q_OFF = 0;
-  static constexpr int K_OFF = 2 * TILE;
+  static constexpr int K_OFF = 2 * Q_TILE;
   static constexpr int V_OFF = K_OFF + STAGES * TILE;
   static constexpr int BAR_OFF = V_OFF + STAGES * TILE;
   static constexpr int SMEM = BAR_OFF + 512 + 1024;
-  static constexpr int ATOM = kKeys * 128;      // bytes of a tile's 64-dim column block (128-byte swizzled rows)
+  static constexpr int O_COL = 2 * KEYS;           // TMEM columns: S (and P over it) of both tiles, O of both
+  static constexpr int TMEM = LONG ? 512 : 256;
 };
 
 struct TcArgs {
@@ -52,6 +64,28 @@ struct TcArgs {
   int vec_q, vec_o;  // 16-byte vectors
   KvDiv page;        // blocks of a page
 };
+
+// Waits for a barrier's phase: true when it completes, false once another role has given up or the limit has passed.
+// The clock is read only after some tries: reading %globaltimer takes longer than most waits here.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, const volatile uint32_t* abort_flag) {
+#pragma unroll 1
+  for (int i = 0; i < 32; ++i)
+    if (mbar_try_wait_long(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait_long(bar, parity))
+    if (*abort_flag || globaltimer() - t0 > kWaitLimitNs) return false;
+  return true;
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok));
+  return ok != 0;
+}
 
 __device__ __forceinline__ uint32_t sw128(int r, int c) {
   return static_cast<uint32_t>(r * 128 + ((((c >> 3) ^ r) & 7) << 4) + ((c & 7) << 1));
@@ -68,25 +102,23 @@ __device__ __forceinline__ uint32_t pack_p(float a, float b) {
   }
 }
 
-// Two FP32 values in one 64-bit register: one instruction adds or multiplies both.
-__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpack_f32x2(uint64_t x) {
+// Two FP32 fused multiply-adds (additions) in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return r;
 }
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
 
@@ -113,12 +145,11 @@ __device__ __forceinline__ uint64_t sdesc_v(uint32_t saddr, uint32_t atom_bytes)
   return d;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK,
-                                                                       const __grid_constant__ CUtensorMap tmV,
-                                                                       const __grid_constant__ KvAttnArgs a,
-                                                                       const __grid_constant__ TcArgs tc) {
-  using C = TcCfg<D>;
+template <typename T, int D, int LONG>
+__global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CTAS))
+    kv_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                           const __grid_constant__ KvAttnArgs a, const __grid_constant__ TcArgs tc) {
+  using C = TcCfg<D, LONG>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
@@ -127,14 +158,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
   uint64_t* v_full = k_free + C::STAGES;
   uint64_t* v_free = v_full + C::STAGES;
   uint64_t* s_full = v_free + C::STAGES;      // [2] MMA → softmax: S of the tile ready
-  uint64_t* p_full = s_full + 2;              // [2] softmax → MMA: P written (128 arrivals)
+  uint64_t* p_full = s_full + 2;              // [2] softmax → MMA: P written (4 warps)
   uint64_t* o_full = p_full + 2;              // [2] MMA → softmax: every product of the tile done
-  uint64_t* q_full = o_full + 2;              // [2] softmax → MMA: Q written (128 arrivals)
+  uint64_t* q_full = o_full + 2;              // [2] softmax → MMA: Q written (4 warps)
   uint64_t* v_raw = q_full + 2;               // [1] TMA → producer: a V tile with hidden rows to clear
   uint64_t* drain = v_raw + 1;                // [1] MMA: products issued before it gave up
   uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile uint32_t* abort_flag = slot + 1;
-  uint32_t* bad_page = slot + 2;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int seq = blockIdx.y;
@@ -149,8 +179,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
   const int base_t = sq.length - sq.n;
   const int t0 = base_t + r0 / group, t1 = base_t + (r0 + rows - 1) / group;
   const KvBlocks kb = kv_blocks(a, t0, t1, tc.shift);
-  const int per = kKeys >> tc.shift;  // blocks of a step
-  const int steps = (kb.n + per - 1) >> (7 - tc.shift);
+  const int per = C::KEYS >> tc.shift;  // blocks of a step
+  const int steps = (kb.n + per - 1) >> (C::LOG_KEYS - tc.shift);
   const int tiles = rows > kRows ? 2 : 1;
   const int* table = a.st.table + seq * a.st.ld_table;
 
@@ -163,37 +193,59 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, kRows);
+      mbar_init(p_full + i, 4);
       mbar_init(o_full + i, 1);
-      mbar_init(q_full + i, kRows);
+      mbar_init(q_full + i, 4);
     }
     mbar_init(v_raw, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
-    *bad_page = 0;
     fence_mbar_init();
   }
   if (warp == 9) {
-    tmem_alloc(slot, 512);
+    tmem_alloc(slot, C::TMEM);
     tmem_relinquish();
     tc_fence_before();
   }
-  __syncthreads();
+  // the warp's 32 rows of Q, 16 bytes a lane and neighbouring lanes in one row
+  constexpr int CH = D / 8;  // 16-byte chunks of a row
+  const int wrow = (warp & 3) * 32;               // the warp's first row of its tile
+  const int w0 = r0 + (warp >> 2) * kRows + wrow;  // and its packed row
+  uint4 qv[CH];
+  if (warp < 8) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int r = w0 + c * (32 / CH) + lane / CH;
+      qv[c] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < r0 + rows) {
+        const int tok = r / group;
+        const T* p = static_cast<const T*>(a.q.p) + (static_cast<long long>(sq.row0) + tok) * a.q.ld +
+                     (kvh * group + r - tok * group) * a.q.hs + 8 * (lane % CH);
+        if (tc.vec_q) {
+          qv[c] = __ldg(reinterpret_cast<const uint4*>(p));
+        } else {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+          qv[c].x = h[0] | static_cast<uint32_t>(h[1]) << 16, qv[c].y = h[2] | static_cast<uint32_t>(h[3]) << 16;
+          qv[c].z = h[4] | static_cast<uint32_t>(h[5]) << 16, qv[c].w = h[6] | static_cast<uint32_t>(h[7]) << 16;
+        }
+      }
+    }
+  }
+  // every page that the tile reads lies in the pool, or the rows go the row-by-row way, which leaves such pages out
+  int bad = 0;
+  for (int x = tid; x < kb.n; x += C::THREADS) {
+    const int id = __ldg(table + tc.page.of(kb.at(x)));
+    bad |= id < 0 || id >= a.c.pages;
+  }
+  const bool good = __syncthreads_or(bad) == 0;
   tc_fence_after();
   const uint32_t tmem = *slot;
-  // every page that the tile reads lies in the pool, or the rows go the row-by-row way, which leaves such pages out
-  for (int x = tid; x < kb.n; x += kTcThreads) {
-    const int id = __ldg(table + tc.page.of(kb.at(x)));
-    if (id < 0 || id >= a.c.pages) *bad_page = 1u;
-  }
-  __syncthreads();
-  const bool good = *bad_page == 0u;
 
   if (good && warp >= 8) {
-   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcRegsIssue));
+   if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
    if (warp == 8) {
     // ---- producer: lane = block (and 64-dim column block) of a step ----
-    const int blk = lane & (per - 1), atom = lane >> (7 - tc.shift);
+    const int blk = lane & (per - 1), atom = lane >> (C::LOG_KEYS - tc.shift);
     const bool mine = atom < D / 64;
     const int size = 1 << tc.shift, first = kv_first(a, t0 < 0 ? 0 : t0);
     const uint32_t off = atom * C::ATOM + blk * (size * 128);
@@ -212,13 +264,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
       const int st = j % C::STAGES;
       const uint32_t ph = (j / C::STAGES) & 1;
       const int next = row_of(j + 1);  // in flight during this step's waits
-      if (!mbar_wait(k_free + st, ph ^ 1) || *abort_flag) ok = false;
+      ok = bar_wait(k_free + st, ph ^ 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (lane == 0) mbar_arrive_expect_tx(k_full + st, C::TILE);
       __syncwarp();
       if (mine) tma_load_2d(smem + C::K_OFF + st * C::TILE + off, &tmK, k_full + st, 64 * atom, row);
-      if (!mbar_wait(v_free + st, ph ^ 1) || *abort_flag) ok = false;
+      ok = bar_wait(v_free + st, ph ^ 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       // keys of the step that no row of the CTA sees: their values, whatever they are, become zeros
@@ -231,7 +283,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
       __syncwarp();
       if (mine) tma_load_2d(vt, &tmV, bar, 64 * atom, row);
       if (clear) {
-        ok = mbar_wait(v_raw, raw_phase);
+        ok = bar_wait(v_raw, raw_phase, abort_flag);
         raw_phase ^= 1;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -264,31 +316,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
     }
    } else if (warp == 9) {
     // ---- MMA issuer ----
-    if (lane == 0 && steps > 0) {
+    // The whole warp runs it, one elected lane issues: what the instructions take stays in uniform registers (with one
+    // lane in a branch of its own, an MMA took 80 clocks to issue).
+    if (steps > 0) {
+      const bool leader = elect_one();
       constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
-      constexpr uint32_t is = idesc_f32acc(fmt, kRows, kKeys);
+      constexpr uint32_t is = idesc_f32acc(fmt, kRows, C::KEYS);
       constexpr uint32_t io = idesc_f32acc(fmt, kRows, D) | (1u << 16);  // B (V) MN-major
       const uint32_t qa = smem_u32(smem + C::Q_OFF), ka = smem_u32(smem + C::K_OFF), va = smem_u32(smem + C::V_OFF);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t ph) {
-        if (ok && (!mbar_wait(bar, ph) || *abort_flag)) ok = false;
+        ok = ok && __all_sync(0xffffffffu, bar_wait(bar, ph, abort_flag));
         return ok;
       };
       auto scores = [&](int i, int j) {  // S_i of step j
-        const uint32_t q = qa + i * C::TILE, k = ka + (j % C::STAGES) * C::TILE;
+        if (!leader) return;
+        const uint32_t q = qa + i * C::Q_TILE, k = ka + (j % C::STAGES) * C::TILE;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d)
-          umma_bf16(tmem + i * kKeys, sdesc_k_sw128(q + (d >> 2) * C::ATOM + 32 * (d & 3)),
+          umma_bf16(tmem + i * C::KEYS, sdesc_k_sw128(q + (d >> 2) * C::Q_ATOM + 32 * (d & 3)),
                     sdesc_k_sw128(k + (d >> 2) * C::ATOM + 32 * (d & 3)), is, d > 0);
         umma_commit(s_full + i);
       };
+      auto commit = [&](uint64_t* bar) {
+        if (leader) umma_commit(bar);
+      };
+      auto values = [&](int i, int j) {  // O_i of step j
+        if (!leader) return;
+        const uint32_t v = va + (j % C::STAGES) * C::TILE;
+#pragma unroll
+        for (int k = 0; k < C::KEYS / 16; ++k)
+          umma_f16_ts(tmem + C::O_COL + i * D, tmem + i * C::KEYS + 8 * k, sdesc_v(v + 2048 * k, C::ATOM), io,
+                      j > 0 || k > 0);
+      };
       wait(k_full, 0);
       for (int i = 0; i < tiles && ok; ++i) {
-        if (!wait(q_full + i, 0)) break;
+        // long walks: tile 1 starts when tile 0 has its first P, and the offset stays: one tile's exponentials run
+        // under the other's products (20,000 keys, 64 dims: 288 -> 256 us)
+        if (!wait(q_full + i, 0) || (C::KEYS == 128 && i == 1 && steps > 24 && !wait(p_full, 0))) break;
         tc_fence_after();
         scores(i, 0);
       }
-      if (ok) umma_commit(k_free);
+      if (ok) commit(k_free);
       for (int j = 0; j < steps && ok; ++j) {
         const int jn = j + 1;
         if (jn < steps) wait(k_full + jn % C::STAGES, (jn / C::STAGES) & 1);
@@ -296,22 +365,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
         for (int i = 0; i < tiles && ok; ++i) {
           if (!wait(p_full + i, j & 1)) break;
           tc_fence_after();
-          const uint32_t v = va + (j % C::STAGES) * C::TILE;
-#pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            umma_f16_ts(tmem + 2 * kKeys + i * D, tmem + i * kKeys + 8 * k, sdesc_v(v + 2048 * k, C::ATOM), io,
-                        j > 0 || k > 0);
+          values(i, j);
           if (jn < steps)
             scores(i, jn);
           else
-            umma_commit(o_full + i);
+            commit(o_full + i);
         }
         if (ok) {
-          umma_commit(v_free + j % C::STAGES);
-          if (jn < steps) umma_commit(k_free + jn % C::STAGES);
+          commit(v_free + j % C::STAGES);
+          if (jn < steps) commit(k_free + jn % C::STAGES);
         }
       }
-      if (!ok) {
+      if (!ok && leader) {
         *abort_flag = 1;
         atomicOr(a.err, kErrAttnWait);
         umma_commit(drain);  // every product issued has completed once this flips
@@ -322,84 +387,52 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
    }
   } else if (good) {
     // ---- softmax: tile i, a thread a row ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcRegsSoftmax));
-    const int i = warp >> 2, row = (warp & 3) * 32 + lane;
+    if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
+    const int i = warp >> 2;
     if (i < tiles) {
-      const int r = r0 + i * kRows + row;
-      const bool mine = r < r0 + rows;
-      const bool any = r0 + i * kRows + (warp & 3) * 32 < r0 + rows;  // the warp has a row
-      const int rr = mine ? r : r0 + rows - 1;
-      const int tok = rr / group, head = kvh * group + rr % group;
-      const int t = base_t + tok, first = kv_first(a, t < 0 ? 0 : t);
-      const long long grow = static_cast<long long>(sq.row0) + tok;
-      const T* qp = static_cast<const T*>(a.q.p) + grow * a.q.ld + head * a.q.hs;
-      uint8_t* qs = smem + C::Q_OFF + i * C::TILE;
+      uint8_t* qs = smem + C::Q_OFF + i * C::Q_TILE;
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (mine) {
-          if (tc.vec_q) {
-            u = __ldg(reinterpret_cast<const uint4*>(qp) + c);
-          } else {
-            const uint16_t* h = reinterpret_cast<const uint16_t*>(qp) + 8 * c;
-            u.x = h[0] | static_cast<uint32_t>(h[1]) << 16, u.y = h[2] | static_cast<uint32_t>(h[3]) << 16;
-            u.z = h[4] | static_cast<uint32_t>(h[5]) << 16, u.w = h[6] | static_cast<uint32_t>(h[7]) << 16;
-          }
-        }
-        *reinterpret_cast<uint4*>(qs + (c >> 3) * C::ATOM + sw128(row, 8 * (c & 7))) = u;
+      for (int c = 0; c < CH; ++c) {
+        const int row = wrow + c * (32 / CH) + lane / CH, ch = lane % CH;
+        *reinterpret_cast<uint4*>(qs + (ch >> 3) * C::Q_ATOM + sw128(row, 8 * (ch & 7))) = qv[c];
       }
       fence_proxy_async_smem();
-      mbar_arrive(q_full + i);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full + i);
 
-      // the warp's tokens
-      const int rw0 = r0 + i * kRows + (warp & 3) * 32, rw1 = min(rw0 + 31, r0 + rows - 1);
-      const int tw0 = base_t + rw0 / group, tw1 = base_t + rw1 / group;
+      const bool any = w0 < r0 + rows;  // the warp has a row
+      const bool mine = w0 + lane < r0 + rows;
+      // the thread's token and the warp's
+      const int w1 = min(w0 + 31, r0 + rows - 1);
+      const int t = base_t + min(w0 + lane, w1) / group, first = kv_first(a, t < 0 ? 0 : t);
+      const int tw0 = base_t + w0 / group, tw1 = base_t + w1 / group;
       const int fw0 = kv_first(a, tw0 < 0 ? 0 : tw0), fw1 = kv_first(a, tw1 < 0 ? 0 : tw1);
-      const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-      const uint32_t s_col = lanes + i * kKeys, o_col = lanes + 2 * kKeys + i * D;
+      const uint32_t lanes = tmem + (static_cast<uint32_t>(wrow) << 16);
+      const uint32_t s_col = lanes + i * C::KEYS, o_col = lanes + C::O_COL + i * D;
       const float sl2 = a.scale * kTcLog2e;
+      // steps open0 .. open1 − 1 lie in the band, and every row of the warp sees every key of them
+      const int to_band = kb.a - kb.b;  // block x of the band is key block x − to_band
+      const int open0 = (max(kb.a, to_band + ((fw1 + (1 << tc.shift) - 1) >> tc.shift)) + per - 1) / per;
+      const int last_open = tw0 + 1 < C::KEYS ? -1 : to_band + ((tw0 + 1 - C::KEYS) >> tc.shift);  // a step's first block
+      const int open1 = last_open < 0 ? 0 : last_open / per + 1;
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
       for (int j = 0; j < steps; ++j) {
-        const bool got = mbar_wait(s_full + i, j & 1) && !*abort_flag;
+        const bool got = bar_wait(s_full + i, j & 1, abort_flag);
         ok = __all_sync(0xffffffffu, got);
         if (!ok) break;
         tc_fence_after();
         if (any) {
-          float s[4][32];
-          uint32_t shut = 0u;  // 32-key chunks that no row of the warp sees
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_col + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s[c]));
-          tmem_ld_wait();
-          // Hide what a row does not see. A step of the band that every row of the warp sees whole skips this.
-          const int key0 = kb.at(j * per) << tc.shift;
-          if (!(j * per >= kb.a && key0 + kKeys - 1 <= tw0 && key0 >= fw1)) {
-            const int sub = tc.shift - 4;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int ha = 8 * j + 2 * c, hc = ha + 1;  // the chunk's two 16-key halves
-              const int ka = (kb.at(ha >> sub) << tc.shift) + ((ha & ((1 << sub) - 1)) << 4);
-              const int kc = (kb.at(hc >> sub) << tc.shift) + ((hc & ((1 << sub) - 1)) << 4);
-              if ((ka > tw1 || (ka + 15 < fw0 && ka >= a.sinks)) && (kc > tw1 || (kc + 15 < fw0 && kc >= a.sinks))) shut |= 1u << c;
-              const uint32_t bits = block_bits(ka, t, first, a.sinks) | block_bits(kc, t, first, a.sinks) << 16;
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((bits >> e) & 1u)) s[c][e] = -INFINITY;
-            }
-          }
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) mx4[(e >> 1) & 3] = fmax3(mx4[(e >> 1) & 3], s[c][e], s[c][e + 1]);
-          const float top = fmax3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * sl2;
-          if (__any_sync(0xffffffffu, top > m + kTcLazy)) {
+          constexpr int NC = C::KEYS / 32;
+          auto load = [&](int c, float (&x)[32]) { tmem_ld_32x32b_x32(s_col + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(x)); };
+          // raises the running maximum to `top` and takes l and O along
+          auto raise = [&](float top) {
             const float mn = fmaxf(m, top);
             const float up = mn == -INFINITY ? 1.0f : kv_ex2(m - mn);
             m = mn;
             l *= up;
             if (j > 0) {
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < D / 32; ++c) {
                 uint32_t o[32];
                 tmem_ld_32x32b_x32(o_col + 32 * c, o);
@@ -409,36 +442,107 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
                 tmem_st_32x32b_x32(o_col + 32 * c, o);
               }
             }
-          }
-          const float base = m == -INFINITY ? 0.0f : m;
-          uint64_t l2[4] = {0ull, 0ull, 0ull, 0ull};  // pairs of partial row sums
-          const uint64_t sc2 = pack_f32x2(sl2, sl2), base2 = pack_f32x2(-base, -base);
+          };
+          float2 ls[2];  // the step's row sum, in four chains
+          // P of a chunk: 2^(x · sl2 − m), its sums in FP32 before the rounding to 16 bits
+          auto probabilities = [&](const float (&x)[32], float base, uint32_t (&pk)[16]) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
-            if ((shut >> c) & 1u) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) pk[e] = 0u;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(s[c][e], s[c][e + 1]), sc2, base2));
-                const float p0 = kv_ex2(x.x), p1 = kv_ex2(x.y);
-                l2[(e >> 1) & 3] = add_f32x2(l2[(e >> 1) & 3], pack_f32x2(p0, p1));
-                pk[e >> 1] = pack_p<T>(p0, p1);
-              }
+            for (int e = 0; e < 32; e += 2) {
+              const float2 y = fma2(make_float2(x[e], x[e + 1]), make_float2(sl2, sl2), make_float2(-base, -base));
+              const float2 p = make_float2(kv_ex2(y.x), kv_ex2(y.y));
+              ls[(e >> 1) & 1] = add2(ls[(e >> 1) & 1], p);
+              pk[e >> 1] = pack_p<T>(p.x, p.y);
             }
-            tmem_st_32x32b_x16(s_col + 16 * c, pk);
+          };
+          auto row_sum = [&] { return (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y); };
+          // A step that every row of the warp sees whole, once there is a maximum to take the exponentials against: the
+          // scores stay in registers. Only where a row's sum then shows that a score had passed the running maximum by
+          // much, the step's own is taken and the exponentials once more. P below 2^14 fits FP16, and its sums FP32.
+          if (C::HOLD && j >= open0 && j < open1 && !__any_sync(0xffffffffu, m == -INFINITY)) {
+            float s[NC][32];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) load(c, s[c]);
+            tmem_ld_wait();
+            for (bool again = false;;) {
+              ls[0] = ls[1] = make_float2(0.0f, 0.0f);
+#pragma unroll
+              for (int c = 0; c < NC; ++c) {
+                uint32_t pk[16];
+                probabilities(s[c], m, pk);
+                tmem_st_32x32b_x16(s_col + 16 * c, pk);
+              }
+              if (again || !__any_sync(0xffffffffu, !(row_sum() <= 16384.0f))) break;
+              again = true;
+              float mx = s[0][0];
+#pragma unroll
+              for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[c][e]);
+              raise(mx * sl2);
+            }
+            l += row_sum();
+          } else {
+            // Any other step, by 32 keys read twice: for the maximum (raised where a score passes it by 2^kLazy), then
+            // for P, with what a row does not see hidden and what no row of the warp sees skipped.
+            const int sub = tc.shift - 4;
+            auto chunk_keys = [&](int c, int& ka, int& kc) {  // first keys of the chunk's two 16-key halves
+              const int ha = 2 * NC * j + 2 * c, hc = ha + 1;
+              ka = (kb.at(ha >> sub) << tc.shift) + ((ha & ((1 << sub) - 1)) << 4);
+              kc = (kb.at(hc >> sub) << tc.shift) + ((hc & ((1 << sub) - 1)) << 4);
+            };
+            auto closed = [&](int k) { return k > tw1 || (k + 15 < fw0 && k >= a.sinks); };
+            auto hide = [&](int ka, int kc, float (&x)[32]) {
+              if (ka + 31 <= tw0 && ka >= fw1 && kc == ka + 16) return;
+              const uint32_t bits = block_bits(ka, t, first, a.sinks) | block_bits(kc, t, first, a.sinks) << 16;
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((bits >> e) & 1u)) x[e] = -INFINITY;
+            };
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+            for (int c = 0; c < NC; ++c) {
+              int ka, kc;
+              chunk_keys(c, ka, kc);
+              if (closed(ka) && closed(kc)) continue;
+              float x[32];
+              load(c, x);
+              tmem_ld_wait();
+              hide(ka, kc, x);
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], x[e], x[e + 1]);
+            }
+            const float top = fmax3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * sl2;
+            if (__any_sync(0xffffffffu, top > m + kTcLazy)) raise(top);
+            const float base = m == -INFINITY ? 0.0f : m;
+            ls[0] = ls[1] = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+            for (int c = 0; c < NC; ++c) {
+              // P over S: chunk c goes over S's columns 16 c .. 16 c + 15, whose chunk (c / 2) has been read by now
+              uint32_t pk[16];
+              int ka, kc;
+              chunk_keys(c, ka, kc);
+              if (closed(ka) && closed(kc)) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) pk[e] = 0u;
+              } else {
+                float x[32];
+                load(c, x);
+                tmem_ld_wait();
+                hide(ka, kc, x);
+                probabilities(x, base, pk);
+              }
+              tmem_st_32x32b_x16(s_col + 16 * c, pk);
+            }
+            l += row_sum();
           }
-          const float2 la = unpack_f32x2(add_f32x2(add_f32x2(l2[0], l2[1]), add_f32x2(l2[2], l2[3])));
-          l += la.x + la.y;
           tmem_st_wait();
         }
         tc_fence_before();
-        mbar_arrive(p_full + i);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + i);
       }
       if (ok) {
-        const bool got = steps == 0 || (mbar_wait(o_full + i, 0) && !*abort_flag);
+        const bool got = steps == 0 || bar_wait(o_full + i, 0, abort_flag);
         ok = __all_sync(0xffffffffu, got);
       }
       if (!ok) {
@@ -446,9 +550,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
         if (lane == 0) atomicOr(a.err, kErrAttnWait);
       } else if (any) {
         tc_fence_after();
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        T* op = static_cast<T*>(a.out.p) + grow * a.out.ld + head * a.out.hs;
+        const float inv = m == -INFINITY || l == 0.0f ? 0.0f : 1.0f / l;  // no maximum: no key seen
         bool nan = l != l;
+        // the row's values through the tile's (consumed) Q into whole-row stores
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -459,23 +563,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0u;
           }
-          if (mine) {
-            uint32_t pk[16];
+          uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float v0 = __uint_as_float(o[e]) * inv, v1 = __uint_as_float(o[e + 1]) * inv;
-              nan |= v0 != v0 || v1 != v1;
-              pk[e >> 1] = kv_pack<T>(v0, v1);
-            }
-            if (tc.vec_o) {
-              uint4* dst = reinterpret_cast<uint4*>(op + 32 * c);
+          for (int e = 0; e < 32; e += 2) {
+            const float v0 = __uint_as_float(o[e]) * inv, v1 = __uint_as_float(o[e + 1]) * inv;
+            nan |= v0 != v0 || v1 != v1;
+            pk[e >> 1] = kv_pack<T>(v0, v1);
+          }
 #pragma unroll
-              for (int u = 0; u < 4; ++u) dst[u] = make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
-            } else {
-              uint16_t* dst = reinterpret_cast<uint16_t*>(op + 32 * c);
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<uint4*>(qs + (c >> 1) * C::Q_ATOM + sw128(wrow + lane, 8 * (4 * (c & 1) + u))) =
+                make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
+        }
+        __syncwarp();
 #pragma unroll
-              for (int u = 0; u < 16; ++u) dst[2 * u] = pk[u] & 0xFFFFu, dst[2 * u + 1] = pk[u] >> 16;
-            }
+        for (int c = 0; c < CH; ++c) {
+          const int row = c * (32 / CH) + lane / CH, ch = lane % CH, r = w0 + row;
+          if (r > w1) continue;
+          const uint4 v = *reinterpret_cast<const uint4*>(qs + (ch >> 3) * C::Q_ATOM + sw128(wrow + row, 8 * (ch & 7)));
+          const int tok = r / group;
+          T* op = static_cast<T*>(a.out.p) + (static_cast<long long>(sq.row0) + tok) * a.out.ld +
+                  (kvh * group + r - tok * group) * a.out.hs + 8 * ch;
+          if (tc.vec_o) {
+            *reinterpret_cast<uint4*>(op) = v;
+          } else {
+            uint16_t* h = reinterpret_cast<uint16_t*>(op);
+            h[0] = v.x & 0xFFFFu, h[1] = v.x >> 16, h[2] = v.y & 0xFFFFu, h[3] = v.y >> 16;
+            h[4] = v.z & 0xFFFFu, h[5] = v.z >> 16, h[6] = v.w & 0xFFFFu, h[7] = v.w >> 16;
           }
         }
         uint32_t redo = __ballot_sync(0xffffffffu, mine && nan);
@@ -483,7 +597,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
         while (redo) {
           const int w = __ffs(redo) - 1;
           redo &= redo - 1;
-          const int xr = rw0 + w, xt = xr / group, xh = kvh * group + xr % group;
+          const int xr = w0 + w, xt = xr / group, xh = kvh * group + xr % group;
           const long long xg = static_cast<long long>(sq.row0) + xt;
           kv_attend_row<T, 16, D>(a, seq, base_t + xt, xh, static_cast<const T*>(a.q.p) + xg * a.q.ld + xh * a.q.hs,
                                   static_cast<T*>(a.out.p) + xg * a.out.ld + xh * a.out.hs);
@@ -491,7 +605,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
       }
     }
   } else {
-    for (int r = warp; r < rows; r += kTcThreads / 32) {
+    for (int r = warp; r < rows; r += C::THREADS / 32) {
       const int xr = r0 + r, xt = xr / group, xh = kvh * group + xr % group;
       const long long xg = static_cast<long long>(sq.row0) + xt;
       kv_attend_row<T, 16, D>(a, seq, base_t + xt, xh, static_cast<const T*>(a.q.p) + xg * a.q.ld + xh * a.q.hs,
@@ -502,13 +616,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attention_tc_kernel(const __
   __syncthreads();
   if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, C::TMEM);
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int LONG>
 cudaError_t launch_tc(const KvAttnArgs& a, cudaStream_t s) {
-  using C = TcCfg<D>;
+  using C = TcCfg<D, LONG>;
   const long long group = a.heads / a.c.kv_heads;
   TcArgs tc{};
   tc.supers = static_cast<int>((a.st.max_new * group + 2 * kRows - 1) / (2 * kRows));
@@ -525,14 +639,16 @@ cudaError_t launch_tc(const KvAttnArgs& a, cudaStream_t s) {
   if (!make_operand_map(&mk, a.c.k, op, tc.pool_rows, D, D, 1 << tc.shift) ||
       !make_operand_map(&mv, a.c.v, op, tc.pool_rows, D, D, 1 << tc.shift))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(kv_attention_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  cudaError_t e = cudaFuncSetAttribute(kv_attention_tc_kernel<T, D, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return e;
   // the warpgroups' shares add up to the launch's registers only if it has this many
-  cudaFuncAttributes at{};
-  if ((e = cudaFuncGetAttributes(&at, kv_attention_tc_kernel<T, D>)) != cudaSuccess) return e;
-  if (at.numRegs != kTcRegs) return cudaErrorInvalidConfiguration;
+  if (C::SPLIT_REGS) {
+    cudaFuncAttributes at{};
+    if ((e = cudaFuncGetAttributes(&at, kv_attention_tc_kernel<T, D, LONG>)) != cudaSuccess) return e;
+    if (at.numRegs != C::REGS) return cudaErrorInvalidConfiguration;
+  }
   const dim3 grid(static_cast<unsigned>(tc.supers) * a.c.kv_heads, a.st.sequences);
-  kv_attention_tc_kernel<T, D><<<grid, kTcThreads, C::SMEM, s>>>(mk, mv, a, tc);
+  kv_attention_tc_kernel<T, D, LONG><<<grid, C::THREADS, C::SMEM, s>>>(mk, mv, a, tc);
   return cudaGetLastError();
 }
 
@@ -544,8 +660,16 @@ bool kv_attention_tc_ok(const KvAttnArgs& a) {
 }
 
 cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, cudaStream_t s) {
-  if (a.c.dim == 64) return a.c.f16 ? launch_tc<__half, 64>(a, s) : launch_tc<__nv_bfloat16, 64>(a, s);
-  return a.c.f16 ? launch_tc<__half, 128>(a, s) : launch_tc<__nv_bfloat16, 128>(a, s);
+  if (a.c.dim == 128) return a.c.f16 ? launch_tc<__half, 128, 1>(a, s) : launch_tc<__nv_bfloat16, 128, 1>(a, s);
+  // Two CTAs an SM where there are that many, or where a walk is a few steps (64 sequences of 130 tokens: 49 against
+  // 78 us; 64 of 1000: 394 against 530 us; 36 of 256 new tokens over 4096: alike); one with longer steps where there are
+  // not (9 of 256 over 20,000, 144 CTAs: 256 against 454 us).
+  const long long keys = a.window > 0 ? std::min<long long>(a.st.max_length, static_cast<long long>(a.window) + a.sinks)
+                                      : a.st.max_length;
+  const long long rows = static_cast<long long>(a.st.max_new) * (a.heads / a.c.kv_heads);
+  const long long ctas = (rows + 2 * kRows - 1) / (2 * kRows) * a.c.kv_heads * a.st.sequences;
+  if (ctas >= 2 * 148 || keys <= 512) return a.c.f16 ? launch_tc<__half, 64, 0>(a, s) : launch_tc<__nv_bfloat16, 64, 0>(a, s);
+  return a.c.f16 ? launch_tc<__half, 64, 1>(a, s) : launch_tc<__nv_bfloat16, 64, 1>(a, s);
 }
 
 }  // namespace jc

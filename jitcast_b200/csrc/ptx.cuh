@@ -92,6 +92,20 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint64
   }
 }
 
+// mbar_try_wait that suspends the thread for up to about a millisecond, for waits whose polling would take issue
+// slots from the SM's other warps.
+__device__ __forceinline__ bool mbar_try_wait_long(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
+}
+
 // ---- TMA --------------------------------------------------------------------------------
 // 2-D tiled bulk-tensor load into this CTA's shared memory, completing on `bar`.
 // x is the innermost (contiguous) coordinate; callers keep x·elem_size a multiple of 16.
