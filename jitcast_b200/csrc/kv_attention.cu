@@ -60,29 +60,27 @@ __device__ __forceinline__ __half2 codes(uint32_t u) {
 
 // The registers of SUB 16-key blocks: lane (g, t) = (lane / 4, lane % 4) has keys g and g + 8 of K (a quarter of the
 // dims each) and keys 2t, 2t + 1, 2t + 8, 2t + 9 of V (an eighth of the dims each).
-template <int BITS, int D>
+template <int BITS, int D, int SUB>
 struct Frag;
 
 template <int D>
-struct Frag<16, D> {
-  static constexpr int SUB = 1;
+struct Frag<16, D, 1> {
   uint4 k[2][D / 32];
   uint4 v[4][D / 64];
 
-  __device__ __forceinline__ void load_k(const KvCache& c, long long row, bool on, int, int g, int t) {
+  __device__ __forceinline__ void load_k(const KvCache& c, long long row, int, int g, int t) {
     const uint4* p = static_cast<const uint4*>(c.k) + (row + g) * (D / 8) + t;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) k[h][i] = on ? __ldg(p + 8 * h * (D / 8) + 4 * i) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < D / 32; ++i) k[h][i] = __ldg(p + 8 * h * (D / 8) + 4 * i);
   }
-  __device__ __forceinline__ void load_v(const KvCache& c, long long row, bool on, int, int g, int t) {
+  __device__ __forceinline__ void load_v(const KvCache& c, long long row, int, int g, int t) {
     const uint4* p = static_cast<const uint4*>(c.v) + (row + 2 * t) * (D / 8) + g;
 #pragma unroll
     for (int h = 0; h < 4; ++h)
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i)
-        v[h][i] = on ? __ldg(p + ((h & 1) + 8 * (h >> 1)) * (D / 8) + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < D / 64; ++i) v[h][i] = __ldg(p + ((h & 1) + 8 * (h >> 1)) * (D / 8) + 8 * i);
   }
   __device__ __forceinline__ void hide_v(int, int h) {
 #pragma unroll
@@ -118,40 +116,39 @@ struct Frag<16, D> {
   static constexpr int v_step = 1;
 };
 
-template <int D>
-struct Frag<4, D> {
-  static constexpr int SUB = D == 64 ? 4 : 2;  // 5 KB of codes and scales in flight a warp
+template <int D, int SUB>
+struct Frag<4, D, SUB> {
   uint32_t k[SUB][2][D / 32];                  // codes of 32 (D = 64: 16) dims from dim t · D / 4
   uint32_t ks[SUB][2];                         // their group's (scale, min)
   uint32_t v[SUB][4][D / 64];                  // codes of 16 (8) dims from dim g · D / 8
   uint32_t vs[SUB][4];
 
-  __device__ __forceinline__ void load_k(const KvCache& c, long long row, bool on, int u, int g, int t) {
+  __device__ __forceinline__ void load_k(const KvCache& c, long long row, int u, int g, int t) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const long long r = row + g + 8 * h;
       if constexpr (D == 128) {
-        const uint4 x = on ? __ldg(static_cast<const uint4*>(c.k) + r * 4 + t) : make_uint4(0u, 0u, 0u, 0u);
+        const uint4 x = __ldg(static_cast<const uint4*>(c.k) + r * 4 + t);
         k[u][h][0] = x.x, k[u][h][1] = x.y, k[u][h][2] = x.z, k[u][h][3] = x.w;
-        ks[u][h] = on ? __ldg(static_cast<const uint32_t*>(c.k_scale) + r * 4 + t) : 0u;
+        ks[u][h] = __ldg(static_cast<const uint32_t*>(c.k_scale) + r * 4 + t);
       } else {
-        const uint2 x = on ? __ldg(static_cast<const uint2*>(c.k) + r * 4 + t) : make_uint2(0u, 0u);
+        const uint2 x = __ldg(static_cast<const uint2*>(c.k) + r * 4 + t);
         k[u][h][0] = x.x, k[u][h][1] = x.y;
-        ks[u][h] = on ? __ldg(static_cast<const uint32_t*>(c.k_scale) + r * 2 + (t >> 1)) : 0u;
+        ks[u][h] = __ldg(static_cast<const uint32_t*>(c.k_scale) + r * 2 + (t >> 1));
       }
     }
   }
-  __device__ __forceinline__ void load_v(const KvCache& c, long long row, bool on, int u, int g, int t) {
+  __device__ __forceinline__ void load_v(const KvCache& c, long long row, int u, int g, int t) {
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
       const long long r = row + 2 * t + (h & 1) + 8 * (h >> 1);
       if constexpr (D == 128) {
-        const uint2 x = on ? __ldg(static_cast<const uint2*>(c.v) + r * 8 + g) : make_uint2(0u, 0u);
+        const uint2 x = __ldg(static_cast<const uint2*>(c.v) + r * 8 + g);
         v[u][h][0] = x.x, v[u][h][1] = x.y;
-        vs[u][h] = on ? __ldg(static_cast<const uint32_t*>(c.v_scale) + r * 4 + (g >> 1)) : 0u;
+        vs[u][h] = __ldg(static_cast<const uint32_t*>(c.v_scale) + r * 4 + (g >> 1));
       } else {
-        v[u][h][0] = on ? __ldg(static_cast<const uint32_t*>(c.v) + r * 8 + g) : 0u;
-        vs[u][h] = on ? __ldg(static_cast<const uint32_t*>(c.v_scale) + r * 2 + (g >> 2)) : 0u;
+        v[u][h][0] = __ldg(static_cast<const uint32_t*>(c.v) + r * 8 + g);
+        vs[u][h] = __ldg(static_cast<const uint32_t*>(c.v_scale) + r * 2 + (g >> 2));
       }
     }
   }
@@ -195,10 +192,11 @@ struct Frag<4, D> {
 
 struct SplitShape {
   int tiles;        // row tiles of a kv head
-  int chunk;        // 16-key blocks that a CTA takes at most
+  int shift;        // 2^shift keys a block
+  int chunk;        // blocks that a CTA takes at most
   int splits;       // CTAs along the longest sequence's keys
   int vec_q, vec_o; // 16-byte vectors of q, 8-byte (4-element) vectors of out
-  KvDiv page;       // 16-key blocks of a page
+  KvDiv page;       // blocks of a page
 };
 
 // The tile's tokens, and where its keys lie.
@@ -208,12 +206,12 @@ struct Tile {
   KvBlocks kb;
 };
 
-__device__ __forceinline__ Tile tile_of(const KvAttnArgs& a, const KvSeq& q, int group, int r0, int most) {
+__device__ __forceinline__ Tile tile_of(const KvAttnArgs& a, const KvSeq& q, int group, int r0, int most, int shift) {
   Tile x;
   x.rows = min(q.n * group - r0, most);
   x.t0 = q.length - q.n + r0 / group;
   x.t1 = q.length - q.n + (r0 + x.rows - 1) / group;
-  x.kb = x.rows > 0 ? kv_blocks(a, x.t0, x.t1, 4) : KvBlocks{0, 0, 0};
+  x.kb = x.rows > 0 ? kv_blocks(a, x.t0, x.t1, shift) : KvBlocks{0, 0, 0};
   return x;
 }
 
@@ -235,12 +233,13 @@ __device__ __forceinline__ void store4(T* p, float4 v, bool vec) {
   }
 }
 
-template <typename T, int BITS, int D, int NT>
+template <typename T, int BITS, int D, int NT, int SUB>
 __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(const __grid_constant__ KvAttnArgs a,
                                                                       const __grid_constant__ SplitShape sh) {
-  using F = Frag<BITS, D>;
+  using F = Frag<BITS, D, SUB>;
   using M = std::conditional_t<BITS == 4, __half, T>;  // the products' type
-  constexpr int ROWS = 8 * NT, SUB = F::SUB, PITCH = D + 4;
+  constexpr int ROWS = 8 * NT, PITCH = D + 4, KEYS = 16 * SUB;  // KEYS: of a block
+  constexpr int SHIFT = SUB == 1 ? 4 : SUB == 2 ? 5 : 6;
   __shared__ float s_o[kWarps][ROWS][PITCH];
   __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
   __shared__ uint32_t s_nan;
@@ -251,7 +250,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(const _
   const KvSeq sq = kv_seq(a.st, a.c.page_size, seq, a.err);
   const int group = a.heads / a.c.kv_heads;
   const int r0 = tile * ROWS;
-  const Tile tl = tile_of(a, sq, group, r0, ROWS);
+  const Tile tl = tile_of(a, sq, group, r0, ROWS, SHIFT);
   if (tl.rows <= 0) return;
   const int x1 = min(tl.kb.n, (split + 1) * sh.chunk), x0 = split * sh.chunk;
   if (x0 >= x1 && split > 0) return;
@@ -322,19 +321,16 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(const _
   }
 
   const int* table = a.st.table + seq * a.st.ld_table;
-  // the pool row of the block x's first key; −1: no such block, or a page outside the pool
-  auto page_id = [&](int x) -> int {
-    if (x >= x1) return -1;
-    const int id = __ldg(table + sh.page.of(tl.kb.at(x)));
+  // the page of block x; −1: no such block, or an entry outside the pool
+  auto page_id = [&](int x) -> int { return x < x1 ? __ldg(table + sh.page.of(tl.kb.at(x))) : -1; };
+  // the pool row of block x's first key in that page
+  auto pool_row = [&](int x, int id) -> long long {
     if (id < 0 || id >= a.c.pages) {
-      if (lane == 0) atomicOr(a.err, kErrKvStep);
+      if (x < x1 && lane == 0) atomicOr(a.err, kErrKvStep);
       return -1;
     }
-    return id;
-  };
-  auto pool_row = [&](int x, int id) -> long long {
     const int b = tl.kb.at(x);
-    const int slot = (b - static_cast<int>(sh.page.of(b)) * static_cast<int>(sh.page.d)) << 4;
+    const int slot = (b - static_cast<int>(sh.page.of(b)) * static_cast<int>(sh.page.d)) << SHIFT;
     return (static_cast<long long>(id) * a.c.kv_heads + kvh) * a.c.page_size + slot;
   };
 
@@ -347,19 +343,25 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(const _
     m[i][0] = m[i][1] = -INFINITY;
     l[i][0] = l[i][1] = 0.0f;
   }
-  // The warp's blocks: SUB at a time, kWarps · SUB apart. A block's K is in flight while the one before it goes
-  // through the softmax and P·V, its V from there to its own P·V, and the page ids one step further ahead.
-  int xb = x0 + warp * SUB;
-  int id[SUB], idn[SUB];
+  // blocks that every row of the tile sees whole need no mask: those from open0 of the band, up to open_t
+  const int open0 = kv_first(a, tl.t1), open_t = tl.t0 - (KEYS - 1);
+  // The warp's blocks, kWarps apart. A block's K is in flight while the one before it goes through the softmax and
+  // P·V, its V from there to its own P·V, and its page id one step further ahead. A block without a page is hidden as
+  // a whole: its registers then hold whatever they held.
+  int x = x0 + warp;
+  long long row = pool_row(x, page_id(x));
+  if (row >= 0) {
 #pragma unroll
-  for (int u = 0; u < SUB; ++u) {
-    id[u] = page_id(xb + u);
-    f.load_k(a.c, id[u] >= 0 ? pool_row(xb + u, id[u]) : 0, id[u] >= 0, u, g, t);
-    f.load_v(a.c, id[u] >= 0 ? pool_row(xb + u, id[u]) : 0, id[u] >= 0, u, g, t);
-    idn[u] = page_id(xb + kWarps * SUB + u);
+    for (int u = 0; u < SUB; ++u) {
+      f.load_k(a.c, row + 16 * u, u, g, t);
+      f.load_v(a.c, row + 16 * u, u, g, t);
+    }
   }
-  for (; xb < x1; xb += kWarps * SUB) {
-    const int xn = xb + kWarps * SUB;
+  int idn = page_id(x + kWarps);
+  for (; x < x1; x += kWarps) {
+    const bool on = row >= 0;
+    row = pool_row(x + kWarps, idn);
+    idn = page_id(x + 2 * kWarps);
     float s[SUB][NT][4];
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
@@ -371,26 +373,29 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(const _
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) MmaT<M>::mma(s[u][i], kf[j], qf[i][j][0], qf[i][j][1]);
       }
-      f.load_k(a.c, idn[u] >= 0 ? pool_row(xn + u, idn[u]) : 0, idn[u] >= 0, u, g, t);
     }
-    // hide what a row does not see; blocks that every row of the tile sees whole skip this
+    if (row >= 0) {
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-      const int key0 = tl.kb.at(xb + u) << 4;
-      const bool open = id[u] >= 0 && key0 + 15 <= tl.t0 && (key0 >= kv_first(a, tl.t1) || key0 + 16 <= a.sinks);
-      if (open) continue;
+      for (int u = 0; u < SUB; ++u) f.load_k(a.c, row + 16 * u, u, g, t);
+    }
+    // hide what a row does not see
+    const int key0 = tl.kb.at(x) << SHIFT;
+    if (!on || key0 > open_t || (key0 < open0 && key0 + KEYS > a.sinks)) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int u = 0; u < SUB; ++u) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = key0 + g + 8 * (e >> 1), tt = tq[i][e & 1];
-          if (id[u] < 0 || j > tt || (j < kv_first(a, tt) && j >= a.sinks)) s[u][i][e] = -INFINITY;
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = key0 + 16 * u + g + 8 * (e >> 1), tt = tq[i][e & 1];
+            if (!on || j > tt || (j < kv_first(a, tt) && j >= a.sinks)) s[u][i][e] = -INFINITY;
+          }
+        // and values that no row sees (slots past the length hold anything)
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int j = key0 + 16 * u + 2 * t + (h & 1) + 8 * (h >> 1);
+          if (!on || j > tl.t1 || (j < kv_first(a, tl.t0) && j >= a.sinks)) f.hide_v(u, h);
         }
-      // and values that no row sees (slots past the length hold anything)
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const int j = key0 + 2 * t + (h & 1) + 8 * (h >> 1);
-        if (j > tl.t1 || (j < kv_first(a, tl.t0) && j >= a.sinks)) f.hide_v(u, h);
       }
     }
     // the running maximum, moved only where a score passes it by 2^kLazy
@@ -447,12 +452,10 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(const _
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) MmaT<M>::mma(o[i][j], vf[j], pf[i][0], pf[i][1]);
-      f.load_v(a.c, idn[u] >= 0 ? pool_row(xn + u, idn[u]) : 0, idn[u] >= 0, u, g, t);
     }
+    if (row >= 0) {
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-      id[u] = idn[u];
-      idn[u] = page_id(xn + kWarps * SUB + u);
+      for (int u = 0; u < SUB; ++u) f.load_v(a.c, row + 16 * u, u, g, t);
     }
   }
 
@@ -535,7 +538,7 @@ __global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__
     bool bad = false;
     if (w < rows) {
       const int r = i * group + head % group;  // its row of the kv head
-      const Tile tl = tile_of(a, sq, group, r / rows_per_tile * rows_per_tile, rows_per_tile);
+      const Tile tl = tile_of(a, sq, group, r / rows_per_tile * rows_per_tile, rows_per_tile, sh.shift);
       if (tl.kb.n > sh.chunk) {
         const int splits = (tl.kb.n + sh.chunk - 1) / sh.chunk;
         const long long row = (static_cast<long long>(sq.row0) + i) * a.heads + head;
@@ -577,22 +580,33 @@ int rows_per_tile(const KvAttnArgs& a) {
   return rows <= 8 ? 8 : 16;
 }
 
-// The most 16-key blocks that a tile reads, and how they are split: enough CTAs for every SM to hold some twice
-// over, of at least 8 blocks a warp (128 keys; a shorter loop is all latency), each split's partial result being a few
-// rows of D floats against chunk · 16 keys of cache.
+// 16-key sub-blocks of a block: a 4-bit cache takes 32 keys (64 at 64 dims) at a time, 5 KB of codes and scales in
+// flight a warp and one page lookup, where a page holds whole blocks of that many.
+int subs_of(const KvAttnArgs& a) {
+  if (a.c.bits == 16) return 1;
+  const int full = a.c.dim == 64 ? 4 : 2;
+  return a.c.page_size % (16 * full) == 0 ? full : 1;
+}
+
+// The most blocks that a tile reads, and how they are split: enough CTAs for every SM to hold some twice over, of at
+// least 128 keys a warp (a shorter loop is all latency), each split's partial result being a few rows of D floats
+// against chunk blocks of cache.
 SplitShape shape_of(const KvAttnArgs& a) {
   const long long group = a.heads / a.c.kv_heads, rpt = rows_per_tile(a);
   SplitShape sh{};
   sh.tiles = static_cast<int>((a.st.max_new * group + rpt - 1) / rpt);
+  const int subs = subs_of(a), size = 16 * subs;
+  sh.shift = subs == 1 ? 4 : subs == 2 ? 5 : 6;
   const long long tokens = (rpt + group - 2) / group + 1;  // most tokens of a tile
   long long keys = a.st.max_length;
-  if (a.window > 0 && a.sinks + static_cast<long long>(a.window) + tokens + 30 < keys)
-    keys = a.sinks + static_cast<long long>(a.window) + tokens + 30;
-  const long long blocks = (keys + 15) / 16;
+  // the sinks' last block, and the band's first and last, may be partial
+  const long long reach = a.sinks + static_cast<long long>(a.window) + tokens + 2 * (size - 1);
+  if (a.window > 0 && reach < keys) keys = reach;
+  const long long blocks = (keys + size - 1) / size;
   const long long items = static_cast<long long>(sh.tiles) * a.c.kv_heads * a.st.sequences;
   const long long want = (148 * 4 * 2 + items - 1) / items;
   long long chunk = (blocks + want - 1) / want;
-  const long long least = 8 * kWarps;
+  const long long least = 128 * kWarps / size;
   if (chunk < least) chunk = least;
   if (blocks <= chunk) chunk = blocks > 0 ? blocks : 1;
   sh.chunk = static_cast<int>(chunk);
@@ -603,8 +617,16 @@ SplitShape shape_of(const KvAttnArgs& a) {
   };
   sh.vec_q = fits(a.q, 16);
   sh.vec_o = fits(a.out, 8);
-  sh.page = KvDiv(static_cast<unsigned>(a.c.page_size / 16));
+  sh.page = KvDiv(static_cast<unsigned>(a.c.page_size / size));
   return sh;
+}
+
+template <typename T, int BITS, int D, int SUB>
+void split(const KvAttnArgs& a, const SplitShape& sh, int rpt, dim3 grid, cudaStream_t s) {
+  if (rpt == 8)
+    kv_attention_split_kernel<T, BITS, D, 1, SUB><<<grid, 32 * kWarps, 0, s>>>(a, sh);
+  else
+    kv_attention_split_kernel<T, BITS, D, 2, SUB><<<grid, 32 * kWarps, 0, s>>>(a, sh);
 }
 
 template <typename T, int BITS, int D>
@@ -612,10 +634,10 @@ cudaError_t attend(const KvAttnArgs& a, cudaStream_t s) {
   const SplitShape sh = shape_of(a);
   const int rpt = rows_per_tile(a);
   const dim3 grid(sh.tiles * a.c.kv_heads, sh.splits, a.st.sequences);
-  if (rpt == 8)
-    kv_attention_split_kernel<T, BITS, D, 1><<<grid, 32 * kWarps, 0, s>>>(a, sh);
+  if (BITS == 4 && sh.shift != 4)
+    split<T, BITS, D, BITS == 16 ? 1 : D == 64 ? 4 : 2>(a, sh, rpt, grid, s);
   else
-    kv_attention_split_kernel<T, BITS, D, 2><<<grid, 32 * kWarps, 0, s>>>(a, sh);
+    split<T, BITS, D, 1>(a, sh, rpt, grid, s);
   if (sh.splits == 1) return cudaGetLastError();
   cudaLaunchConfig_t cfg{};
   const long long rows = static_cast<long long>(a.st.max_new) * a.heads;
