@@ -30,6 +30,8 @@ namespace jc {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kCtas = 148 * 4 * 2;     // CTAs that a call is split into where its rows alone are fewer
+constexpr int kMaxSplits = kCtas;
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's running maximum moves only when a score passes it by this much (as a power of two): probabilities then
 // reach 2^8, which costs no precision in any of the types, and most blocks rescale nothing.
@@ -234,7 +236,7 @@ __device__ __forceinline__ void store4(T* p, float4 v, bool vec) {
 }
 
 template <typename T, int BITS, int D, int NT, int SUB>
-__global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(const __grid_constant__ KvAttnArgs a,
+__global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 2 : BITS == 4 ? 4 : 3) kv_attention_split_kernel(const __grid_constant__ KvAttnArgs a,
                                                                       const __grid_constant__ SplitShape sh) {
   using F = Frag<BITS, D, SUB>;
   using M = std::conditional_t<BITS == 4, __half, T>;  // the products' type
@@ -459,6 +461,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(const _
     }
   }
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // join the warps
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -519,59 +522,71 @@ __global__ void __launch_bounds__(32 * kWarps) kv_attention_split_kernel(const _
     }
 }
 
-// Joins the splits of each output row: D / 4 lanes a row, the splits in order. HBM / L2 bound: it reads what the
-// splits wrote once; launched early (programmatic dependent launch), it waits for them on the device.
+// Joins the splits of an output row: a block a row, D / 4 threads a split at a time, the splits' weights first and
+// their sums in a fixed order. It reads what the splits wrote once. Launched under the splits' end (programmatic
+// dependent launch), it waits for them on the device.
 template <typename T, int BITS, int D>
 __global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__ KvAttnArgs a,
                                                          const __grid_constant__ SplitShape sh, int rows_per_tile) {
-  constexpr int LANES = D / 4;
-  const int lane = threadIdx.x & 31;
-  const int seq = blockIdx.y;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const KvSeq sq = kv_seq(a.st, a.c.page_size, seq, a.err);
+  constexpr int LANES = D / 4, WAYS = 128 / LANES;
+  __shared__ float s_c[kMaxSplits], s_red[8];
+  __shared__ float4 s_acc[WAYS][LANES];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const KvSeq sq = kv_seq(a.st, a.c.page_size, blockIdx.y, a.err);
   const int group = a.heads / a.c.kv_heads;
-  const long long rows = static_cast<long long>(sq.n) * a.heads;
-  // a warp takes 32 / LANES rows; every lane of it stays in the loop for the vote
-  for (long long w0 = (blockIdx.x * 4LL + (threadIdx.x >> 5)) * (32 / LANES); w0 < rows; w0 += gridDim.x * 4LL * (32 / LANES)) {
-    const long long w = w0 + lane / LANES;
-    const int i = static_cast<int>(w / a.heads), head = static_cast<int>(w - static_cast<long long>(i) * a.heads);
-    bool bad = false;
-    if (w < rows) {
-      const int r = i * group + head % group;  // its row of the kv head
-      const Tile tl = tile_of(a, sq, group, r / rows_per_tile * rows_per_tile, rows_per_tile, sh.shift);
-      if (tl.kb.n > sh.chunk) {
-        const int splits = (tl.kb.n + sh.chunk - 1) / sh.chunk;
-        const long long row = (static_cast<long long>(sq.row0) + i) * a.heads + head;
-        const int d = 4 * (lane % LANES);
-        float mm = -INFINITY;
-        for (int k = 0; k < splits; ++k) mm = fmaxf(mm, part_ml(a, sh.splits, k, row, D)->x);
-        const float base = mm == -INFINITY ? 0.0f : mm;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float sum = 0.0f;
+  const int i = blockIdx.x / a.heads, head = blockIdx.x - i * a.heads;
+  const int r = i * group + head % group;  // its row of the kv head
+  const Tile tl = tile_of(a, sq, group, r / rows_per_tile * rows_per_tile, rows_per_tile, sh.shift);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (i >= sq.n || tl.kb.n <= sh.chunk) return;  // one split wrote the row itself
+  const int splits = (tl.kb.n + sh.chunk - 1) / sh.chunk;
+  const long long row = (static_cast<long long>(sq.row0) + i) * a.heads + head;
+  float mm = -INFINITY;
+  for (int k = tid; k < splits; k += 128) mm = fmaxf(mm, part_ml(a, sh.splits, k, row, D)->x);
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, w));
+  if (lane == 0) s_red[warp] = mm;
+  __syncthreads();
+  mm = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  const float base = mm == -INFINITY ? 0.0f : mm;
+  float sum = 0.0f;
+  for (int k = tid; k < splits; k += 128) {
+    const float2 ml = *part_ml(a, sh.splits, k, row, D);
+    const float c = kv_ex2(ml.x - base);
+    s_c[k] = c;
+    sum = fmaf(ml.y, c, sum);
+  }
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+  if (lane == 0) s_red[4 + warp] = sum;
+  __syncthreads();
+  sum = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
+  const int way = tid / LANES, d = tid % LANES;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-        for (int k = 0; k < splits; ++k) {
-          const float2 ml = *part_ml(a, sh.splits, k, row, D);
-          const float4 v = *reinterpret_cast<const float4*>(part_o(a, k, row, D) + d);
-          const float c = kv_ex2(ml.x - base);
-          acc.x = fmaf(v.x, c, acc.x), acc.y = fmaf(v.y, c, acc.y), acc.z = fmaf(v.z, c, acc.z), acc.w = fmaf(v.w, c, acc.w);
-          sum = fmaf(ml.y, c, sum);
-        }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-        bad = acc.x != acc.x || acc.y != acc.y || acc.z != acc.z || acc.w != acc.w;
-        store4(static_cast<T*>(a.out.p) + (static_cast<long long>(sq.row0) + i) * a.out.ld + head * a.out.hs + d, acc, sh.vec_o);
-      }
+  for (int k = way; k < splits; k += WAYS) {
+    const float4 v = *reinterpret_cast<const float4*>(part_o(a, k, row, D) + 4 * d);
+    const float c = s_c[k];
+    acc.x = fmaf(v.x, c, acc.x), acc.y = fmaf(v.y, c, acc.y), acc.z = fmaf(v.z, c, acc.z), acc.w = fmaf(v.w, c, acc.w);
+  }
+  s_acc[way][d] = acc;
+  __syncthreads();
+  bool bad = false;
+  if (tid < LANES) {
+#pragma unroll
+    for (int w = 1; w < WAYS; ++w) {
+      const float4 v = s_acc[w][d];
+      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
     }
-    const uint32_t any = __ballot_sync(0xffffffffu, bad);
-    for (int h = 0; h < 32 / LANES; ++h)
-      if ((any >> (h * LANES)) & (LANES == 32 ? 0xffffffffu : 0xffffu)) {
-        const long long x = w0 + h;
-        const int xi = static_cast<int>(x / a.heads), xh = static_cast<int>(x - static_cast<long long>(xi) * a.heads);
-        const long long row = static_cast<long long>(sq.row0) + xi;
-        kv_attend_row<T, BITS, D>(a, seq, sq.length - sq.n + xi, xh,
-                                  static_cast<const T*>(a.q.p) + row * a.q.ld + xh * a.q.hs,
-                                  static_cast<T*>(a.out.p) + row * a.out.ld + xh * a.out.hs);
-      }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+    bad = acc.x != acc.x || acc.y != acc.y || acc.z != acc.z || acc.w != acc.w;
+    store4(static_cast<T*>(a.out.p) + (static_cast<long long>(sq.row0) + i) * a.out.ld + head * a.out.hs + 4 * d, acc, sh.vec_o);
+  }
+  if (__syncthreads_or(bad) && warp == 0) {
+    const long long g = static_cast<long long>(sq.row0) + i;
+    kv_attend_row<T, BITS, D>(a, blockIdx.y, sq.length - sq.n + i, head, static_cast<const T*>(a.q.p) + g * a.q.ld + head * a.q.hs,
+                              static_cast<T*>(a.out.p) + g * a.out.ld + head * a.out.hs);
   }
 }
 
@@ -604,7 +619,7 @@ SplitShape shape_of(const KvAttnArgs& a) {
   if (a.window > 0 && reach < keys) keys = reach;
   const long long blocks = (keys + size - 1) / size;
   const long long items = static_cast<long long>(sh.tiles) * a.c.kv_heads * a.st.sequences;
-  const long long want = (148 * 4 * 2 + items - 1) / items;
+  const long long want = (kCtas + items - 1) / items;  // at most kMaxSplits
   long long chunk = (blocks + want - 1) / want;
   const long long least = 128 * kWarps / size;
   if (chunk < least) chunk = least;
@@ -641,9 +656,7 @@ cudaError_t attend(const KvAttnArgs& a, cudaStream_t s) {
   if (sh.splits == 1) return cudaGetLastError();
   cudaLaunchConfig_t cfg{};
   const long long rows = static_cast<long long>(a.st.max_new) * a.heads;
-  const long long per = 4 * (32 / (D / 4));
-  const long long blocks = (rows + per - 1) / per;
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks < 65535 ? blocks : 65535), a.st.sequences);
+  cfg.gridDim = dim3(static_cast<unsigned>(rows), a.st.sequences);
   cfg.blockDim = dim3(128);
   cfg.stream = s;
   cudaLaunchAttribute at{};

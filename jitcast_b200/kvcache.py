@@ -179,16 +179,18 @@ class PagedCache:
 
     def _rows(self, t, name, heads=None, tokens=None, dtype=None):
         """jc_kv_rows of t [tokens, heads, head_dim]."""
-        if t.dim() != 3 or t.shape[2] != self.head_dim or t.stride(2) != 1 or t.device != self.device:
-            raise ValueError(f"{name} must be [tokens, heads, {self.head_dim}] on {self.device} with unit stride in "
-                             f"its last dimension, not {tuple(t.shape)} on {t.device}")
-        if heads is not None and t.shape[1] != heads:
-            raise ValueError(f"{name} has {t.shape[1]} heads, not {heads}")
-        if tokens is not None and t.shape[0] != tokens:
-            raise ValueError(f"{name} has {t.shape[0]} tokens, not {tokens}")
+        shape = t.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or t.device != self.device:
+            raise ValueError(f"{name} must be [tokens, heads, {self.head_dim}] on {self.device}, not {tuple(shape)} on {t.device}")
+        ld, hs, one = t.stride()
+        if one != 1:
+            raise ValueError(f"{name} must have unit stride in its last dimension")
+        if heads is not None and shape[1] != heads:
+            raise ValueError(f"{name} has {shape[1]} heads, not {heads}")
+        if tokens is not None and shape[0] != tokens:
+            raise ValueError(f"{name} has {shape[0]} tokens, not {tokens}")
         if dtype is not None and t.dtype != dtype:
             raise ValueError(f"{name} is {t.dtype}, not {dtype}")
-        ld, hs, _ = t.stride()
         return ctypes.byref(_Rows(t.data_ptr(), ld, hs))
 
     def _precision(self, t) -> int:
@@ -229,7 +231,7 @@ class PagedCache:
             heads = q.shape[1] if q.dim() == 3 else 0
             rq = self._rows(q, "q", None, n, dt)
             if q_out is None:
-                q_out = torch.empty((n, heads, self.head_dim), dtype=dt, device=self.device)
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             ro = self._rows(q_out, "q_out", heads, n, dt)
         elif q_out is not None:
             raise ValueError("q_out without q")
@@ -260,7 +262,7 @@ class PagedCache:
         rq = self._rows(q, "q")
         n, heads, dim = q.shape
         if out is None:
-            out = torch.empty((n, heads, dim), dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         ro = self._rows(out, "out", heads, n, q.dtype)
         c_step = step._c(n)
         lib = _lib.lib()
