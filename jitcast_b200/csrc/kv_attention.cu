@@ -49,17 +49,6 @@ __device__ __forceinline__ uint32_t hi16(uint32_t a, uint32_t b) { return __byte
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
-// Codes at bits 0..3 and 16..19 (HIGH: 4..7 and 20..23) of u as FP16: (1024 + c) − 1024, or (1024 + 16 c) / 16 − 64,
-// both exact.
-template <bool HIGH>
-__device__ __forceinline__ __half2 codes(uint32_t u) {
-  const uint32_t x = (u & (HIGH ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
-  if constexpr (HIGH)
-    return __hfma2(u2h(x), u2h(0x2C002C00u), u2h(0xD400D400u));  // 1/16, −64
-  else
-    return __hsub2(u2h(x), u2h(0x64006400u));
-}
-
 // The registers of SUB 16-key blocks: lane (g, t) = (lane / 4, lane % 4) has keys g and g + 8 of K (a quarter of the
 // dims each) and keys 2t, 2t + 1, 2t + 8, 2t + 9 of V (an eighth of the dims each).
 template <int BITS, int D, int SUB>
@@ -163,10 +152,10 @@ struct Frag<4, D, SUB> {
 #pragma unroll
       for (int w = 0; w < D / 32; ++w) {
         const uint32_t x = k[u][h][w], y = x >> 8;
-        f[2 * w][h] = h2u(__hfma2(codes<false>(x), s, m));
-        f[2 * w][h + 2] = h2u(__hfma2(codes<true>(x), s, m));
-        f[2 * w + 1][h] = h2u(__hfma2(codes<false>(y), s, m));
-        f[2 * w + 1][h + 2] = h2u(__hfma2(codes<true>(y), s, m));
+        f[2 * w][h] = h2u(__hfma2(kv_codes<false>(x), s, m));
+        f[2 * w][h + 2] = h2u(__hfma2(kv_codes<true>(x), s, m));
+        f[2 * w + 1][h] = h2u(__hfma2(kv_codes<false>(y), s, m));
+        f[2 * w + 1][h + 2] = h2u(__hfma2(kv_codes<true>(y), s, m));
       }
     }
   }
@@ -180,10 +169,10 @@ struct Frag<4, D, SUB> {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {  // dims 0..3, then 4..7 of the word
           const uint32_t x = e ? hi16(a, b) : lo16(a, b), y = x >> 8;
-          f[4 * w][2 * h + e] = h2u(__hfma2(codes<false>(x), s, m));
-          f[4 * w + 1][2 * h + e] = h2u(__hfma2(codes<true>(x), s, m));
-          f[4 * w + 2][2 * h + e] = h2u(__hfma2(codes<false>(y), s, m));
-          f[4 * w + 3][2 * h + e] = h2u(__hfma2(codes<true>(y), s, m));
+          f[4 * w][2 * h + e] = h2u(__hfma2(kv_codes<false>(x), s, m));
+          f[4 * w + 1][2 * h + e] = h2u(__hfma2(kv_codes<true>(x), s, m));
+          f[4 * w + 2][2 * h + e] = h2u(__hfma2(kv_codes<false>(y), s, m));
+          f[4 * w + 3][2 * h + e] = h2u(__hfma2(kv_codes<true>(y), s, m));
         }
       }
     }

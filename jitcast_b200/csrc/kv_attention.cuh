@@ -72,6 +72,19 @@ __device__ __noinline__ void kv_attend_row(const KvAttnArgs& a, int s, int t, in
   for (int i = 0; i < N; ++i) out[lane + 32 * i] = kv_round<T>(o[i] * inv);
 }
 
+// Codes at bits 0..3 and 16..19 (HIGH: 4..7 and 20..23) of u as FP16: (1024 + c) − 1024, or (1024 + 16 c) / 16 − 64,
+// both exact.
+template <bool HIGH>
+__device__ __forceinline__ __half2 kv_codes(uint32_t u) {
+  const uint32_t x = (u & (HIGH ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
+  const uint32_t c1 = 0x64006400u, c2 = 0x2C002C00u, c3 = 0xD400D400u;  // 1024; 1/16, −64
+  const __half2 h = *reinterpret_cast<const __half2*>(&x);
+  if constexpr (HIGH)
+    return __hfma2(h, *reinterpret_cast<const __half2*>(&c2), *reinterpret_cast<const __half2*>(&c3));
+  else
+    return __hsub2(h, *reinterpret_cast<const __half2*>(&c1));
+}
+
 // 2^x by the special-function unit: 2 ulp, flushes subnormal results (a probability below 2^-126 is none).
 __device__ __forceinline__ float kv_ex2(float x) {
   float y;

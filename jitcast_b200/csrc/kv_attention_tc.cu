@@ -29,11 +29,12 @@ namespace {
 constexpr int kRows = 128;   // rows of a tile (TMEM lanes)
 constexpr float kTcLog2e = 1.4426950408889634f;
 constexpr float kTcLazy = 8.0f;
+constexpr int kUnpack = 3;   // warps that unpack a 4-bit cache's tiles
 
 // LONG 0 (64 dims): 64 keys a step, so that S and O of both tiles take 256 TMEM columns and two CTAs fit on an SM: a
 // CTA's start and end run under the other's steps.
 // LONG 1: 128 keys a step and one CTA an SM; its softmax warps hold their rows' 128 scores, for which the third
-// warpgroup gives up registers (168 a thread at launch: 2 · 208 + 88 = 3 · 168).
+// warpgroup gives up registers (168 a thread at launch: 2 · 208 + 88 = 2 · 192 + 120 = 3 · 168).
 template <int D, int LONG>
 struct TcCfg {
   static_assert(LONG || D == 64, "the short form is for 64 dims");
@@ -43,6 +44,7 @@ struct TcCfg {
   static constexpr int THREADS = LONG ? 384 : 320;
   static constexpr bool SPLIT_REGS = LONG, HOLD = LONG;
   static constexpr int REGS = 168, REGS_SOFTMAX = 208, REGS_ISSUE = 88;
+  static constexpr int REGS_SOFTMAX4 = 192, REGS_UNPACK = 120;  // a 4-bit cache
   static constexpr int STAGES = LONG && D == 128 ? 2 : 4;
   static constexpr int Q_TILE = kRows * D * 2;     // bytes of a Q (and at the end an output) tile
   static constexpr int TILE = KEYS * D * 2;        // bytes of a K or V tile
@@ -52,7 +54,8 @@ struct TcCfg {
   static constexpr int K_OFF = 2 * Q_TILE;
   static constexpr int V_OFF = K_OFF + STAGES * TILE;
   static constexpr int BAR_OFF = V_OFF + STAGES * TILE;
-  static constexpr int SMEM = BAR_OFF + 512 + 1024;
+  static constexpr int MUL_OFF = BAR_OFF + 512;    // 4 bits: what each row's q was divided by
+  static constexpr int SMEM = MUL_OFF + 2 * kRows * 4 + 1024;
   static constexpr int O_COL = 2 * KEYS;           // TMEM columns: S (and P over it) of both tiles, O of both
   static constexpr int TMEM = LONG ? 512 : 256;
 };
@@ -145,11 +148,89 @@ __device__ __forceinline__ uint64_t sdesc_v(uint32_t saddr, uint32_t atom_bytes)
   return d;
 }
 
-template <typename T, int D, int LONG>
+// The producers over a 4-bit cache: kUnpack warps load a step's codes and scales, and write the FP16 values that they
+// stand for as the swizzled K and V tiles. A lane takes 32 dims (one group) of a key: 16 bytes of codes, one (scale, min),
+// four 16-byte stores. While a K tile is unpacked the V tile's codes are in flight, and the next K's under the V tile.
+// Within each 8 dims the values lie in the order 0, 4, 1, 5, 2, 6, 3, 7, as they come out of a word of codes: Q is written
+// in that order too, and the output's columns are put back at the end. Keys that no row sees become zeros.
+template <int D, typename C>
+__device__ __forceinline__ void unpack_tiles(const KvAttnArgs& a, const TcArgs& tc, const KvBlocks& kb, const int* table,
+                                             int kvh, int steps, int t0, int t1, uint8_t* smem, uint64_t* k_full,
+                                             uint64_t* k_free, uint64_t* v_full, uint64_t* v_free,
+                                             volatile uint32_t* abort_flag, int part, int lane) {
+  constexpr int TASKS = C::KEYS * (D / 32), ROUNDS = (TASKS + 32 * kUnpack - 1) / (32 * kUnpack);
+  struct Codes {
+    uint4 c[ROUNDS];
+    uint32_t sm[ROUNDS];  // 0: a key that no row sees
+  };
+  const int size = 1 << tc.shift, first = kv_first(a, t0);
+  auto load = [&](int j, const void* pool, const void* scale, Codes& x) {
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int task = (r * kUnpack + part) * 32 + lane, key = task / (D / 32), grp = task % (D / 32);
+      const int b = j * (C::KEYS >> tc.shift) + (key >> tc.shift);
+      x.c[r] = make_uint4(0u, 0u, 0u, 0u);
+      x.sm[r] = 0u;
+      if (task < TASKS && b < kb.n) {
+        const int kblk = kb.at(b), in = key & (size - 1), idx = (kblk << tc.shift) + in;
+        if (idx <= t1 && (idx >= first || idx < a.sinks)) {
+          const unsigned pg = tc.page.of(kblk);
+          const long long row = (static_cast<long long>(__ldg(table + pg)) * a.c.kv_heads + kvh) * a.c.page_size +
+                                ((kblk - static_cast<int>(pg * tc.page.d)) << tc.shift) + in;
+          x.c[r] = __ldg(static_cast<const uint4*>(pool) + row * (D / 32) + grp);
+          x.sm[r] = __ldg(static_cast<const uint32_t*>(scale) + row * (D / 32) + grp);
+        }
+      }
+    }
+  };
+  auto unpack = [&](const Codes& x, uint8_t* tile) {
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int task = (r * kUnpack + part) * 32 + lane, key = task / (D / 32), grp = task % (D / 32);
+      if (task >= TASKS) continue;
+      const __half2 s = __low2half2(*reinterpret_cast<const __half2*>(&x.sm[r])), m = __high2half2(*reinterpret_cast<const __half2*>(&x.sm[r]));
+      const uint32_t w[4] = {x.c[r].x, x.c[r].y, x.c[r].z, x.c[r].w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int ch = 4 * grp + q;
+        const __half2 h[4] = {__hfma2(kv_codes<false>(w[q]), s, m), __hfma2(kv_codes<true>(w[q]), s, m),
+                              __hfma2(kv_codes<false>(w[q] >> 8), s, m), __hfma2(kv_codes<true>(w[q] >> 8), s, m)};
+        *reinterpret_cast<uint4*>(tile + (ch >> 3) * C::ATOM + sw128(key, 8 * (ch & 7))) = *reinterpret_cast<const uint4*>(h);
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+  };
+  Codes k, v;
+  bool ok = true;
+  if (steps > 0) load(0, a.c.k, a.c.k_scale, k);
+  for (int j = 0; j < steps; ++j) {
+    const int st = j % C::STAGES;
+    const uint32_t ph = ((j / C::STAGES) & 1) ^ 1;
+    load(j, a.c.v, a.c.v_scale, v);
+    ok = __all_sync(0xffffffffu, bar_wait(k_free + st, ph, abort_flag));
+    if (!ok) break;
+    unpack(k, smem + C::K_OFF + st * C::TILE);
+    if (lane == 0) mbar_arrive(k_full + st);
+    if (j + 1 < steps) load(j + 1, a.c.k, a.c.k_scale, k);
+    ok = __all_sync(0xffffffffu, bar_wait(v_free + st, ph, abort_flag));
+    if (!ok) break;
+    unpack(v, smem + C::V_OFF + st * C::TILE);
+    if (lane == 0) mbar_arrive(v_full + st);
+  }
+  if (!ok && lane == 0) {
+    *abort_flag = 1;
+    atomicOr(a.err, kErrAttnWait);
+  }
+}
+
+template <typename T, int BITS, int D, int LONG>
 __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CTAS))
     kv_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                            const __grid_constant__ KvAttnArgs a, const __grid_constant__ TcArgs tc) {
   using C = TcCfg<D, LONG>;
+  using M = std::conditional_t<BITS == 4, __half, T>;  // the products' type
+  static_assert(BITS == 16 || LONG, "a 4-bit cache takes the long form");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
@@ -186,9 +267,9 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
 
   if (tid == 0) {
     for (int i = 0; i < C::STAGES; ++i) {
-      mbar_init(k_full + i, 1);
+      mbar_init(k_full + i, BITS == 4 ? kUnpack : 1);
       mbar_init(k_free + i, 1);
-      mbar_init(v_full + i, 1);
+      mbar_init(v_full + i, BITS == 4 ? kUnpack : 1);
       mbar_init(v_free + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -242,8 +323,13 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
   const uint32_t tmem = *slot;
 
   if (good && warp >= 8) {
-   if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
-   if (warp == 8) {
+   if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BITS == 4 ? C::REGS_UNPACK : C::REGS_ISSUE));
+   if (BITS == 4 && warp != 9) {
+    if constexpr (BITS == 4) {
+      unpack_tiles<D, C>(a, tc, kb, table, kvh, steps, t0 < 0 ? 0 : t0, t1, smem, k_full, k_free, v_full, v_free, abort_flag,
+                         warp == 8 ? 0 : warp - 9, lane);
+    }
+   } else if (BITS == 16 && warp == 8) {
     // ---- producer: lane = block (and 64-dim column block) of a step ----
     const int blk = lane & (per - 1), atom = lane >> (C::LOG_KEYS - tc.shift);
     const bool mine = atom < D / 64;
@@ -320,7 +406,7 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
     // lane in a branch of its own, an MMA took 80 clocks to issue).
     if (steps > 0) {
       const bool leader = elect_one();
-      constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+      constexpr uint32_t fmt = std::is_same<M, __half>::value ? 0u : 1u;
       constexpr uint32_t is = idesc_f32acc(fmt, kRows, C::KEYS);
       constexpr uint32_t io = idesc_f32acc(fmt, kRows, D) | (1u << 16);  // B (V) MN-major
       const uint32_t qa = smem_u32(smem + C::Q_OFF), ka = smem_u32(smem + C::K_OFF), va = smem_u32(smem + C::V_OFF);
@@ -387,14 +473,29 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
    }
   } else if (good) {
     // ---- softmax: tile i, a thread a row ----
-    if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
+    if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BITS == 4 ? C::REGS_SOFTMAX4 : C::REGS_SOFTMAX));
     const int i = warp >> 2;
     if (i < tiles) {
       uint8_t* qs = smem + C::Q_OFF + i * C::Q_TILE;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const int row = wrow + c * (32 / CH) + lane / CH, ch = lane % CH;
-        *reinterpret_cast<uint4*>(qs + (ch >> 3) * C::Q_ATOM + sw128(row, 8 * (ch & 7))) = qv[c];
+        uint4 u = qv[c];
+        if constexpr (BITS == 4) {
+          // FP16, divided by the power of two of the row's largest element (BF16's range does not matter then), in the
+          // order of dims that the unpacked keys have: (0, 4), (1, 5), (2, 6), (3, 7) of each 8
+          const float2 f0 = kv_unpack<T>(u.x), f1 = kv_unpack<T>(u.y), f2 = kv_unpack<T>(u.z), f3 = kv_unpack<T>(u.w);
+          float most = fmaxf(fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))),
+                             fmaxf(fmaxf(fabsf(f2.x), fabsf(f2.y)), fmaxf(fabsf(f3.x), fabsf(f3.y))));
+#pragma unroll
+          for (int w = 1; w < CH; w <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
+          const uint32_t eb = __float_as_uint(most) & 0x7F800000u;
+          const float mul = eb != 0u && eb != 0x7F800000u ? __uint_as_float(eb) : 1.0f, inv = 1.0f / mul;
+          u = make_uint4(pack_p<__half>(f0.x * inv, f2.x * inv), pack_p<__half>(f0.y * inv, f2.y * inv),
+                         pack_p<__half>(f1.x * inv, f3.x * inv), pack_p<__half>(f1.y * inv, f3.y * inv));
+          if (ch == 0) reinterpret_cast<float*>(smem + C::MUL_OFF)[i * kRows + row] = mul;
+        }
+        *reinterpret_cast<uint4*>(qs + (ch >> 3) * C::Q_ATOM + sw128(row, 8 * (ch & 7))) = u;
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -409,7 +510,7 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
       const int fw0 = kv_first(a, tw0 < 0 ? 0 : tw0), fw1 = kv_first(a, tw1 < 0 ? 0 : tw1);
       const uint32_t lanes = tmem + (static_cast<uint32_t>(wrow) << 16);
       const uint32_t s_col = lanes + i * C::KEYS, o_col = lanes + C::O_COL + i * D;
-      const float sl2 = a.scale * kTcLog2e;
+      const float sl2 = a.scale * kTcLog2e * (BITS == 4 ? reinterpret_cast<const float*>(smem + C::MUL_OFF)[i * kRows + wrow + lane] : 1.0f);
       // steps open0 .. open1 − 1 lie in the band, and every row of the warp sees every key of them
       const int to_band = kb.a - kb.b;  // block x of the band is key block x − to_band
       const int open0 = (max(kb.a, to_band + ((fw1 + (1 << tc.shift) - 1) >> tc.shift)) + per - 1) / per;
@@ -451,7 +552,7 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
               const float2 y = fma2(make_float2(x[e], x[e + 1]), make_float2(sl2, sl2), make_float2(-base, -base));
               const float2 p = make_float2(kv_ex2(y.x), kv_ex2(y.y));
               ls[(e >> 1) & 1] = add2(ls[(e >> 1) & 1], p);
-              pk[e >> 1] = pack_p<T>(p.x, p.y);
+              pk[e >> 1] = pack_p<M>(p.x, p.y);
             }
           };
           auto row_sum = [&] { return (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y); };
@@ -566,7 +667,9 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float v0 = __uint_as_float(o[e]) * inv, v1 = __uint_as_float(o[e + 1]) * inv;
+            // the columns of dims e, e + 1 (4 bits: unpacked values lie in the order 0, 4, 1, 5, 2, 6, 3, 7)
+            const int c0 = BITS == 16 ? e : (e & ~7) + (e & 4 ? 1 : 0) + (e & 2 ? 4 : 0), c1 = BITS == 16 ? e + 1 : c0 + 2;
+            const float v0 = __uint_as_float(o[c0]) * inv, v1 = __uint_as_float(o[c1]) * inv;
             nan |= v0 != v0 || v1 != v1;
             pk[e >> 1] = kv_pack<T>(v0, v1);
           }
@@ -599,7 +702,7 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
           redo &= redo - 1;
           const int xr = w0 + w, xt = xr / group, xh = kvh * group + xr % group;
           const long long xg = static_cast<long long>(sq.row0) + xt;
-          kv_attend_row<T, 16, D>(a, seq, base_t + xt, xh, static_cast<const T*>(a.q.p) + xg * a.q.ld + xh * a.q.hs,
+          kv_attend_row<T, BITS, D>(a, seq, base_t + xt, xh, static_cast<const T*>(a.q.p) + xg * a.q.ld + xh * a.q.hs,
                                   static_cast<T*>(a.out.p) + xg * a.out.ld + xh * a.out.hs);
         }
       }
@@ -608,7 +711,7 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
     for (int r = warp; r < rows; r += C::THREADS / 32) {
       const int xr = r0 + r, xt = xr / group, xh = kvh * group + xr % group;
       const long long xg = static_cast<long long>(sq.row0) + xt;
-      kv_attend_row<T, 16, D>(a, seq, base_t + xt, xh, static_cast<const T*>(a.q.p) + xg * a.q.ld + xh * a.q.hs,
+      kv_attend_row<T, BITS, D>(a, seq, base_t + xt, xh, static_cast<const T*>(a.q.p) + xg * a.q.ld + xh * a.q.hs,
                               static_cast<T*>(a.out.p) + xg * a.out.ld + xh * a.out.hs);
     }
   }
@@ -620,7 +723,7 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
   }
 }
 
-template <typename T, int D, int LONG>
+template <typename T, int BITS, int D, int LONG>
 cudaError_t launch_tc(const KvAttnArgs& a, cudaStream_t s) {
   using C = TcCfg<D, LONG>;
   const long long group = a.heads / a.c.kv_heads;
@@ -634,21 +737,21 @@ cudaError_t launch_tc(const KvAttnArgs& a, cudaStream_t s) {
   tc.vec_o = fits(a.out);
   tc.shift = a.c.page_size % 64 == 0 ? 6 : a.c.page_size % 32 == 0 ? 5 : 4;
   tc.page = KvDiv(static_cast<unsigned>(a.c.page_size >> tc.shift));
-  CUtensorMap mk, mv;
+  CUtensorMap mk{}, mv{};
   const int op = std::is_same<T, __half>::value ? kOpF16 : kOpBF16;
-  if (!make_operand_map(&mk, a.c.k, op, tc.pool_rows, D, D, 1 << tc.shift) ||
-      !make_operand_map(&mv, a.c.v, op, tc.pool_rows, D, D, 1 << tc.shift))
+  if (BITS == 16 && (!make_operand_map(&mk, a.c.k, op, tc.pool_rows, D, D, 1 << tc.shift) ||
+                     !make_operand_map(&mv, a.c.v, op, tc.pool_rows, D, D, 1 << tc.shift)))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(kv_attention_tc_kernel<T, D, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  cudaError_t e = cudaFuncSetAttribute(kv_attention_tc_kernel<T, BITS, D, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return e;
   // the warpgroups' shares add up to the launch's registers only if it has this many
   if (C::SPLIT_REGS) {
     cudaFuncAttributes at{};
-    if ((e = cudaFuncGetAttributes(&at, kv_attention_tc_kernel<T, D, LONG>)) != cudaSuccess) return e;
+    if ((e = cudaFuncGetAttributes(&at, kv_attention_tc_kernel<T, BITS, D, LONG>)) != cudaSuccess) return e;
     if (at.numRegs != C::REGS) return cudaErrorInvalidConfiguration;
   }
   const dim3 grid(static_cast<unsigned>(tc.supers) * a.c.kv_heads, a.st.sequences);
-  kv_attention_tc_kernel<T, D, LONG><<<grid, C::THREADS, C::SMEM, s>>>(mk, mv, a, tc);
+  kv_attention_tc_kernel<T, BITS, D, LONG><<<grid, C::THREADS, C::SMEM, s>>>(mk, mv, a, tc);
   return cudaGetLastError();
 }
 
@@ -656,11 +759,15 @@ cudaError_t launch_tc(const KvAttnArgs& a, cudaStream_t s) {
 
 // Rows from which the tensor-core tiles are used: a 128-row tile costs the same for one row as for all.
 bool kv_attention_tc_ok(const KvAttnArgs& a) {
-  return a.c.bits == 16 && static_cast<long long>(a.st.max_new) * (a.heads / a.c.kv_heads) > 32;
+  return static_cast<long long>(a.st.max_new) * (a.heads / a.c.kv_heads) > 32;
 }
 
 cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, cudaStream_t s) {
-  if (a.c.dim == 128) return a.c.f16 ? launch_tc<__half, 128, 1>(a, s) : launch_tc<__nv_bfloat16, 128, 1>(a, s);
+  if (a.c.bits == 4) {
+    if (a.c.dim == 128) return a.c.f16 ? launch_tc<__half, 4, 128, 1>(a, s) : launch_tc<__nv_bfloat16, 4, 128, 1>(a, s);
+    return a.c.f16 ? launch_tc<__half, 4, 64, 1>(a, s) : launch_tc<__nv_bfloat16, 4, 64, 1>(a, s);
+  }
+  if (a.c.dim == 128) return a.c.f16 ? launch_tc<__half, 16, 128, 1>(a, s) : launch_tc<__nv_bfloat16, 16, 128, 1>(a, s);
   // Two CTAs an SM where there are that many, or where a walk is a few steps (64 sequences of 130 tokens: 49 against
   // 78 us; 64 of 1000: 394 against 530 us; 36 of 256 new tokens over 4096: alike); one with longer steps where there are
   // not (9 of 256 over 20,000, 144 CTAs: 256 against 454 us).
@@ -668,8 +775,8 @@ cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, cudaStream_t s) {
                                       : a.st.max_length;
   const long long rows = static_cast<long long>(a.st.max_new) * (a.heads / a.c.kv_heads);
   const long long ctas = (rows + 2 * kRows - 1) / (2 * kRows) * a.c.kv_heads * a.st.sequences;
-  if (ctas >= 2 * 148 || keys <= 512) return a.c.f16 ? launch_tc<__half, 64, 0>(a, s) : launch_tc<__nv_bfloat16, 64, 0>(a, s);
-  return a.c.f16 ? launch_tc<__half, 64, 1>(a, s) : launch_tc<__nv_bfloat16, 64, 1>(a, s);
+  if (ctas >= 2 * 148 || keys <= 512) return a.c.f16 ? launch_tc<__half, 16, 64, 0>(a, s) : launch_tc<__nv_bfloat16, 16, 64, 0>(a, s);
+  return a.c.f16 ? launch_tc<__half, 16, 64, 1>(a, s) : launch_tc<__nv_bfloat16, 16, 64, 1>(a, s);
 }
 
 }  // namespace jc
