@@ -224,13 +224,15 @@ __device__ __forceinline__ void store4(T* p, float4 v, bool vec) {
   }
 }
 
-template <typename T, int BITS, int D, int NT, int SUB>
+template <typename T, int BITS, int D, int NT, int SUB, bool WHOLE>
 __global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 2 : BITS == 4 ? 4 : 3) kv_attention_split_kernel(const __grid_constant__ KvAttnArgs a,
                                                                       const __grid_constant__ SplitShape sh) {
   using F = Frag<BITS, D, SUB>;
   using M = std::conditional_t<BITS == 4, __half, T>;  // the products' type
-  constexpr int ROWS = 8 * NT, PITCH = D + 4, KEYS = 16 * SUB;  // KEYS: of a block
-  constexpr int SHIFT = SUB == 1 ? 4 : SUB == 2 ? 5 : 6;
+  constexpr int ROWS = 8 * NT, PITCH = D + 4;
+  // A step takes SUB 16-key sub-blocks: one block in one page (WHOLE), or SUB blocks that may lie in pages of their own
+  constexpr int PAGES = WHOLE ? 1 : SUB, PER = SUB / PAGES, KEYS = 16 * PER;  // KEYS: of a block
+  constexpr int SHIFT = PER == 1 ? 4 : PER == 2 ? 5 : 6, STEP = kWarps * PAGES;
   __shared__ float s_o[kWarps][ROWS][PITCH];
   __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
   __shared__ uint32_t s_nan;
@@ -336,23 +338,32 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 2 : BITS == 4 ? 4 : 3) 
   }
   // blocks that every row of the tile sees whole need no mask: those from open0 of the band, up to open_t
   const int open0 = kv_first(a, tl.t1), open_t = tl.t0 - (KEYS - 1);
-  // The warp's blocks, kWarps apart. A block's K is in flight while the one before it goes through the softmax and
-  // P·V, its V from there to its own P·V, and its page id one step further ahead. A block without a page is hidden as
-  // a whole: its registers then hold whatever they held.
-  int x = x0 + warp;
-  long long row = pool_row(x, page_id(x));
-  if (row >= 0) {
+  // The warp's steps, kWarps apart. A step's K is in flight while the one before it goes through the softmax and P·V,
+  // its V from there to its own P·V, and its page ids one step further ahead. A block without a page is hidden as a
+  // whole: its registers then hold whatever they held.
+  int x = x0 + warp * PAGES;
+  long long row[PAGES];
+  int idn[PAGES];
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-      f.load_k(a.c, row + 16 * u, u, g, t);
-      f.load_v(a.c, row + 16 * u, u, g, t);
+  for (int p = 0; p < PAGES; ++p) {
+    row[p] = pool_row(x + p, page_id(x + p));
+    if (row[p] >= 0) {
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        f.load_k(a.c, row[p] + 16 * u, p * PER + u, g, t);
+        f.load_v(a.c, row[p] + 16 * u, p * PER + u, g, t);
+      }
     }
+    idn[p] = page_id(x + STEP + p);
   }
-  int idn = page_id(x + kWarps);
-  for (; x < x1; x += kWarps) {
-    const bool on = row >= 0;
-    row = pool_row(x + kWarps, idn);
-    idn = page_id(x + 2 * kWarps);
+  for (; x < x1; x += STEP) {
+    uint32_t on = 0u;
+#pragma unroll
+    for (int p = 0; p < PAGES; ++p) {
+      on |= row[p] >= 0 ? 1u << p : 0u;
+      row[p] = pool_row(x + STEP + p, idn[p]);
+      idn[p] = page_id(x + 2 * STEP + p);
+    }
     float s[SUB][NT][4];
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
@@ -365,27 +376,33 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 2 : BITS == 4 ? 4 : 3) 
         for (int j = 0; j < D / 16; ++j) MmaT<M>::mma(s[u][i], kf[j], qf[i][j][0], qf[i][j][1]);
       }
     }
-    if (row >= 0) {
 #pragma unroll
-      for (int u = 0; u < SUB; ++u) f.load_k(a.c, row + 16 * u, u, g, t);
-    }
+    for (int p = 0; p < PAGES; ++p)
+      if (row[p] >= 0) {
+#pragma unroll
+        for (int u = 0; u < PER; ++u) f.load_k(a.c, row[p] + 16 * u, p * PER + u, g, t);
+      }
     // hide what a row does not see
-    const int key0 = tl.kb.at(x) << SHIFT;
-    if (!on || key0 > open_t || (key0 < open0 && key0 + KEYS > a.sinks)) {
 #pragma unroll
-      for (int u = 0; u < SUB; ++u) {
+    for (int p = 0; p < PAGES; ++p) {
+      const int key0 = tl.kb.at(x + p) << SHIFT;
+      const bool here = (on >> p) & 1u;
+      if (here && key0 <= open_t && (key0 >= open0 || key0 + KEYS <= a.sinks)) continue;
+#pragma unroll
+      for (int w = 0; w < PER; ++w) {
+        const int u = p * PER + w, k0 = key0 + 16 * w;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int j = key0 + 16 * u + g + 8 * (e >> 1), tt = tq[i][e & 1];
-            if (!on || j > tt || (j < kv_first(a, tt) && j >= a.sinks)) s[u][i][e] = -INFINITY;
+            const int j = k0 + g + 8 * (e >> 1), tt = tq[i][e & 1];
+            if (!here || j > tt || (j < kv_first(a, tt) && j >= a.sinks)) s[u][i][e] = -INFINITY;
           }
         // and values that no row sees (slots past the length hold anything)
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
-          const int j = key0 + 16 * u + 2 * t + (h & 1) + 8 * (h >> 1);
-          if (!on || j > tl.t1 || (j < kv_first(a, tl.t0) && j >= a.sinks)) f.hide_v(u, h);
+          const int j = k0 + 2 * t + (h & 1) + 8 * (h >> 1);
+          if (!here || j > tl.t1 || (j < kv_first(a, tl.t0) && j >= a.sinks)) f.hide_v(u, h);
         }
       }
     }
@@ -444,10 +461,12 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 2 : BITS == 4 ? 4 : 3) 
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) MmaT<M>::mma(o[i][j], vf[j], pf[i][0], pf[i][1]);
     }
-    if (row >= 0) {
 #pragma unroll
-      for (int u = 0; u < SUB; ++u) f.load_v(a.c, row + 16 * u, u, g, t);
-    }
+    for (int p = 0; p < PAGES; ++p)
+      if (row[p] >= 0) {
+#pragma unroll
+        for (int u = 0; u < PER; ++u) f.load_v(a.c, row[p] + 16 * u, p * PER + u, g, t);
+      }
   }
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -584,13 +603,13 @@ int rows_per_tile(const KvAttnArgs& a) {
   return rows <= 8 ? 8 : 16;
 }
 
-// 16-key sub-blocks of a block: a 4-bit cache takes 32 keys (64 at 64 dims) at a time, 5 KB of codes and scales in
-// flight a warp and one page lookup, where a page holds whole blocks of that many.
-int subs_of(const KvAttnArgs& a) {
-  if (a.c.bits == 16) return 1;
-  const int full = a.c.dim == 64 ? 4 : 2;
-  return a.c.page_size % (16 * full) == 0 ? full : 1;
-}
+// 16-key sub-blocks of a step: a 4-bit cache takes 32 keys (64 at 64 dims) at a time, 5 KB of codes and scales in
+// flight a warp; one page lookup for all of them where a page holds whole steps, else one each.
+template <int BITS, int D>
+constexpr int kSubs = BITS == 16 ? 1 : D == 64 ? 4 : 2;
+
+int subs_of(const KvAttnArgs& a) { return a.c.bits == 16 ? 1 : a.c.dim == 64 ? 4 : 2; }
+bool whole_steps(const KvAttnArgs& a) { return a.c.page_size % (16 * subs_of(a)) == 0; }
 
 // The most blocks that a tile reads, and how they are split: enough CTAs for every SM to hold some twice over, of at
 // least 128 keys a warp (a shorter loop is all latency), each split's partial result being a few rows of D floats
@@ -599,7 +618,7 @@ SplitShape shape_of(const KvAttnArgs& a) {
   const long long group = a.heads / a.c.kv_heads, rpt = rows_per_tile(a);
   SplitShape sh{};
   sh.tiles = static_cast<int>((a.st.max_new * group + rpt - 1) / rpt);
-  const int subs = subs_of(a), size = 16 * subs;
+  const int subs = whole_steps(a) ? subs_of(a) : 1, size = 16 * subs;  // of a block
   sh.shift = subs == 1 ? 4 : subs == 2 ? 5 : 6;
   const long long tokens = (rpt + group - 2) / group + 1;  // most tokens of a tile
   long long keys = a.st.max_length;
@@ -625,12 +644,13 @@ SplitShape shape_of(const KvAttnArgs& a) {
   return sh;
 }
 
-template <typename T, int BITS, int D, int SUB>
+template <typename T, int BITS, int D, bool WHOLE>
 void split(const KvAttnArgs& a, const SplitShape& sh, int rpt, dim3 grid, cudaStream_t s) {
+  constexpr int SUB = kSubs<BITS, D>;
   if (rpt == 8)
-    kv_attention_split_kernel<T, BITS, D, 1, SUB><<<grid, 32 * kWarps, 0, s>>>(a, sh);
+    kv_attention_split_kernel<T, BITS, D, 1, SUB, WHOLE><<<grid, 32 * kWarps, 0, s>>>(a, sh);
   else
-    kv_attention_split_kernel<T, BITS, D, 2, SUB><<<grid, 32 * kWarps, 0, s>>>(a, sh);
+    kv_attention_split_kernel<T, BITS, D, 2, SUB, WHOLE><<<grid, 32 * kWarps, 0, s>>>(a, sh);
 }
 
 template <typename T, int BITS, int D>
@@ -638,10 +658,10 @@ cudaError_t attend(const KvAttnArgs& a, cudaStream_t s) {
   const SplitShape sh = shape_of(a);
   const int rpt = rows_per_tile(a);
   const dim3 grid(sh.tiles * a.c.kv_heads, sh.splits, a.st.sequences);
-  if (BITS == 4 && sh.shift != 4)
-    split<T, BITS, D, BITS == 16 ? 1 : D == 64 ? 4 : 2>(a, sh, rpt, grid, s);
+  if (BITS == 16 || whole_steps(a))
+    split<T, BITS, D, true>(a, sh, rpt, grid, s);
   else
-    split<T, BITS, D, 1>(a, sh, rpt, grid, s);
+    split<T, BITS, D, BITS == 16>(a, sh, rpt, grid, s);
   if (sh.splits == 1) return cudaGetLastError();
   cudaLaunchConfig_t cfg{};
   const long long rows = static_cast<long long>(a.st.max_new) * a.heads;

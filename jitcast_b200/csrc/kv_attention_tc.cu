@@ -29,22 +29,22 @@ namespace {
 constexpr int kRows = 128;   // rows of a tile (TMEM lanes)
 constexpr float kTcLog2e = 1.4426950408889634f;
 constexpr float kTcLazy = 8.0f;
-constexpr int kUnpack = 3;   // warps that unpack a 4-bit cache's tiles
+constexpr int kUnpack = 7;   // warps that unpack a 4-bit cache's tiles (8 and 10 to 15)
 
 // LONG 0 (64 dims): 64 keys a step, so that S and O of both tiles take 256 TMEM columns and two CTAs fit on an SM: a
 // CTA's start and end run under the other's steps.
-// LONG 1: 128 keys a step and one CTA an SM; its softmax warps hold their rows' 128 scores, for which the third
-// warpgroup gives up registers (168 a thread at launch: 2 · 208 + 88 = 2 · 192 + 120 = 3 · 168).
-template <int D, int LONG>
+// LONG 1: 128 keys a step and one CTA an SM; its softmax warps hold their rows' 128 scores, for which the other
+// warpgroups give up registers: of 168 a thread at launch, 2 · 208 + 88 = 3 · 168; over a 4-bit cache, with a fourth
+// warpgroup for the unpacking, of 128, 2 · 184 + 2 · 72 = 4 · 128.
+template <int BITS, int D, int LONG>
 struct TcCfg {
   static_assert(LONG || D == 64, "the short form is for 64 dims");
   static constexpr int KEYS = LONG ? 128 : 64;     // keys of a step
   static constexpr int LOG_KEYS = LONG ? 7 : 6;
   static constexpr int CTAS = LONG ? 1 : 2;        // on an SM
-  static constexpr int THREADS = LONG ? 384 : 320;
+  static constexpr int THREADS = BITS == 4 ? 512 : LONG ? 384 : 320;
   static constexpr bool SPLIT_REGS = LONG, HOLD = LONG;
-  static constexpr int REGS = 168, REGS_SOFTMAX = 208, REGS_ISSUE = 88;
-  static constexpr int REGS_SOFTMAX4 = 192, REGS_UNPACK = 120;  // a 4-bit cache
+  static constexpr int REGS = BITS == 4 ? 128 : 168, REGS_SOFTMAX = BITS == 4 ? 184 : 208, REGS_ISSUE = BITS == 4 ? 72 : 88;
   static constexpr int STAGES = LONG && D == 128 ? 2 : 4;
   static constexpr int Q_TILE = kRows * D * 2;     // bytes of a Q (and at the end an output) tile
   static constexpr int TILE = KEYS * D * 2;        // bytes of a K or V tile
@@ -163,24 +163,24 @@ __device__ __forceinline__ void unpack_tiles(const KvAttnArgs& a, const TcArgs& 
     uint4 c[ROUNDS];
     uint32_t sm[ROUNDS];  // 0: a key that no row sees
   };
-  const int size = 1 << tc.shift, first = kv_first(a, t0);
-  auto load = [&](int j, const void* pool, const void* scale, Codes& x) {
+  const int size = 1 << tc.shift, per = C::KEYS >> tc.shift, first = kv_first(a, t0);
+  // pool row of the lane's block of step j (lanes 0 .. per − 1), fetched a step ahead of its codes
+  auto row_of = [&](int j) -> int {
+    const int b = j * per + lane;
+    if (lane >= per || b >= kb.n) return 0;
+    const int kblk = kb.at(b);
+    const unsigned pg = tc.page.of(kblk);
+    return (__ldg(table + pg) * a.c.kv_heads + kvh) * a.c.page_size + ((kblk - static_cast<int>(pg * tc.page.d)) << tc.shift);
+  };
+  auto load = [&](int j, int rows, const void* pool, const void* scale, Codes& x) {
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
       const int task = (r * kUnpack + part) * 32 + lane, key = task / (D / 32), grp = task % (D / 32);
-      const int b = j * (C::KEYS >> tc.shift) + (key >> tc.shift);
-      x.c[r] = make_uint4(0u, 0u, 0u, 0u);
-      x.sm[r] = 0u;
-      if (task < TASKS && b < kb.n) {
-        const int kblk = kb.at(b), in = key & (size - 1), idx = (kblk << tc.shift) + in;
-        if (idx <= t1 && (idx >= first || idx < a.sinks)) {
-          const unsigned pg = tc.page.of(kblk);
-          const long long row = (static_cast<long long>(__ldg(table + pg)) * a.c.kv_heads + kvh) * a.c.page_size +
-                                ((kblk - static_cast<int>(pg * tc.page.d)) << tc.shift) + in;
-          x.c[r] = __ldg(static_cast<const uint4*>(pool) + row * (D / 32) + grp);
-          x.sm[r] = __ldg(static_cast<const uint32_t*>(scale) + row * (D / 32) + grp);
-        }
-      }
+      const int b = j * per + (key >> tc.shift), in = key & (size - 1), idx = (kb.at(b) << tc.shift) + in;
+      const long long row = __shfl_sync(0xffffffffu, rows, (key >> tc.shift) & 31) + in;
+      const bool on = task < TASKS && b < kb.n && idx <= t1 && (idx >= first || idx < a.sinks);
+      x.c[r] = on ? __ldg(static_cast<const uint4*>(pool) + row * (D / 32) + grp) : make_uint4(0u, 0u, 0u, 0u);
+      x.sm[r] = on ? __ldg(static_cast<const uint32_t*>(scale) + row * (D / 32) + grp) : 0u;
     }
   };
   auto unpack = [&](const Codes& x, uint8_t* tile) {
@@ -189,10 +189,13 @@ __device__ __forceinline__ void unpack_tiles(const KvAttnArgs& a, const TcArgs& 
       const int task = (r * kUnpack + part) * 32 + lane, key = task / (D / 32), grp = task % (D / 32);
       if (task >= TASKS) continue;
       const __half2 s = __low2half2(*reinterpret_cast<const __half2*>(&x.sm[r])), m = __high2half2(*reinterpret_cast<const __half2*>(&x.sm[r]));
-      const uint32_t w[4] = {x.c[r].x, x.c[r].y, x.c[r].z, x.c[r].w};
+      // groups 2 and 3 (the other column block, same banks) store their words in the order 2, 3, 0, 1
+      const bool turn = (grp & 2) != 0;
+      const uint32_t w[4] = {turn ? x.c[r].z : x.c[r].x, turn ? x.c[r].w : x.c[r].y, turn ? x.c[r].x : x.c[r].z,
+                             turn ? x.c[r].y : x.c[r].w};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int ch = 4 * grp + q;
+        const int ch = 4 * grp + (q ^ (grp & 2));
         const __half2 h[4] = {__hfma2(kv_codes<false>(w[q]), s, m), __hfma2(kv_codes<true>(w[q]), s, m),
                               __hfma2(kv_codes<false>(w[q] >> 8), s, m), __hfma2(kv_codes<true>(w[q] >> 8), s, m)};
         *reinterpret_cast<uint4*>(tile + (ch >> 3) * C::ATOM + sw128(key, 8 * (ch & 7))) = *reinterpret_cast<const uint4*>(h);
@@ -203,16 +206,19 @@ __device__ __forceinline__ void unpack_tiles(const KvAttnArgs& a, const TcArgs& 
   };
   Codes k, v;
   bool ok = true;
-  if (steps > 0) load(0, a.c.k, a.c.k_scale, k);
+  int rows = row_of(0), rows_n = row_of(1);
+  load(0, rows, a.c.k, a.c.k_scale, k);
   for (int j = 0; j < steps; ++j) {
     const int st = j % C::STAGES;
     const uint32_t ph = ((j / C::STAGES) & 1) ^ 1;
-    load(j, a.c.v, a.c.v_scale, v);
+    load(j, rows, a.c.v, a.c.v_scale, v);
+    rows = rows_n;
+    rows_n = row_of(j + 2);
     ok = __all_sync(0xffffffffu, bar_wait(k_free + st, ph, abort_flag));
     if (!ok) break;
     unpack(k, smem + C::K_OFF + st * C::TILE);
     if (lane == 0) mbar_arrive(k_full + st);
-    if (j + 1 < steps) load(j + 1, a.c.k, a.c.k_scale, k);
+    load(j + 1, rows, a.c.k, a.c.k_scale, k);  // past the last step: nothing is seen, nothing read
     ok = __all_sync(0xffffffffu, bar_wait(v_free + st, ph, abort_flag));
     if (!ok) break;
     unpack(v, smem + C::V_OFF + st * C::TILE);
@@ -225,10 +231,10 @@ __device__ __forceinline__ void unpack_tiles(const KvAttnArgs& a, const TcArgs& 
 }
 
 template <typename T, int BITS, int D, int LONG>
-__global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CTAS))
+__global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, D, LONG>::CTAS))
     kv_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                            const __grid_constant__ KvAttnArgs a, const __grid_constant__ TcArgs tc) {
-  using C = TcCfg<D, LONG>;
+  using C = TcCfg<BITS, D, LONG>;
   using M = std::conditional_t<BITS == 4, __half, T>;  // the products' type
   static_assert(BITS == 16 || LONG, "a 4-bit cache takes the long form");
   extern __shared__ uint8_t smem_raw[];
@@ -323,7 +329,7 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
   const uint32_t tmem = *slot;
 
   if (good && warp >= 8) {
-   if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BITS == 4 ? C::REGS_UNPACK : C::REGS_ISSUE));
+   if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
    if (BITS == 4 && warp != 9) {
     if constexpr (BITS == 4) {
       unpack_tiles<D, C>(a, tc, kb, table, kvh, steps, t0 < 0 ? 0 : t0, t1, smem, k_full, k_free, v_full, v_free, abort_flag,
@@ -473,7 +479,7 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
    }
   } else if (good) {
     // ---- softmax: tile i, a thread a row ----
-    if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BITS == 4 ? C::REGS_SOFTMAX4 : C::REGS_SOFTMAX));
+    if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
     const int i = warp >> 2;
     if (i < tiles) {
       uint8_t* qs = smem + C::Q_OFF + i * C::Q_TILE;
@@ -725,7 +731,7 @@ __global__ void __launch_bounds__((TcCfg<D, LONG>::THREADS), (TcCfg<D, LONG>::CT
 
 template <typename T, int BITS, int D, int LONG>
 cudaError_t launch_tc(const KvAttnArgs& a, cudaStream_t s) {
-  using C = TcCfg<D, LONG>;
+  using C = TcCfg<BITS, D, LONG>;
   const long long group = a.heads / a.c.kv_heads;
   TcArgs tc{};
   tc.supers = static_cast<int>((a.st.max_new * group + 2 * kRows - 1) / (2 * kRows));
