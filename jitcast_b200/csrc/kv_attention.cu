@@ -30,8 +30,10 @@ namespace jc {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kCtas = 148 * 4 * 2;     // CTAs that a call is split into where its rows alone are fewer
-constexpr int kMaxSplits = kCtas;
+// CTAs that a call is split into where its rows alone are fewer: one wave of equal ones for one sequence (131,000 keys
+// over 4 bits: 52 us, 56 with two waves, 66 with four), many small ones for sequences of any lengths (48 of 5000 to 32,500
+// keys: 332 us, 367 with two waves).
+constexpr int kCtasOne = 148 * 4, kCtasMany = 148 * 16, kMaxSplits = kCtasMany;
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's running maximum moves only when a score passes it by this much (as a power of two): probabilities then
 // reach 2^8, which costs no precision in any of the types, and most blocks rescale nothing.
@@ -627,7 +629,7 @@ SplitShape shape_of(const KvAttnArgs& a) {
   if (a.window > 0 && reach < keys) keys = reach;
   const long long blocks = (keys + size - 1) / size;
   const long long items = static_cast<long long>(sh.tiles) * a.c.kv_heads * a.st.sequences;
-  const long long want = (kCtas + items - 1) / items;  // at most kMaxSplits
+  const long long want = ((a.st.sequences == 1 ? kCtasOne : kCtasMany) + items - 1) / items;  // at most kMaxSplits
   long long chunk = (blocks + want - 1) / want;
   const long long least = 128 * kWarps / size;
   if (chunk < least) chunk = least;

@@ -295,23 +295,37 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
     tc_fence_before();
   }
   // the warp's 32 rows of Q, 16 bytes a lane and neighbouring lanes in one row
-  constexpr int CH = D / 8;  // 16-byte chunks of a row
+  constexpr int CH = D / 8, RPI = 32 / CH;  // 16-byte chunks of a row, rows of one round
   const int wrow = (warp & 3) * 32;               // the warp's first row of its tile
   const int w0 = r0 + (warp >> 2) * kRows + wrow;  // and its packed row
+  const int ch = lane % CH;
+  // the lane's rows w0 + lane / CH, + RPI, ..: token and head of the group, without a division each
+  struct RowWalk {
+    int tok, rem, dt, dr, group;
+    __device__ __forceinline__ RowWalk(int r, int step, int g) : tok(r / g), rem(r % g), dt(step / g), dr(step % g), group(g) {}
+    __device__ __forceinline__ void next() {
+      tok += dt;
+      rem += dr;
+      if (rem >= group) rem -= group, ++tok;
+    }
+  };
   uint4 qv[CH];
   if (warp < 8) {
+    RowWalk at(w0 + lane / CH, RPI, group);
+    const T* base = static_cast<const T*>(a.q.p) + sq.row0 * a.q.ld + kvh * group * a.q.hs + 8 * ch;
+    if (tc.vec_q) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int r = w0 + c * (32 / CH) + lane / CH;
-      qv[c] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < r0 + rows) {
-        const int tok = r / group;
-        const T* p = static_cast<const T*>(a.q.p) + (static_cast<long long>(sq.row0) + tok) * a.q.ld +
-                     (kvh * group + r - tok * group) * a.q.hs + 8 * (lane % CH);
-        if (tc.vec_q) {
-          qv[c] = __ldg(reinterpret_cast<const uint4*>(p));
-        } else {
-          const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+      for (int c = 0; c < CH; ++c, at.next()) {
+        const bool on = w0 + c * RPI + lane / CH < r0 + rows;  // a row past the last reads the first one, and is zeroed
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(base + (on ? at.tok * a.q.ld + at.rem * a.q.hs : 0)));
+        qv[c] = make_uint4(on ? u.x : 0u, on ? u.y : 0u, on ? u.z : 0u, on ? u.w : 0u);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < CH; ++c, at.next()) {
+        qv[c] = make_uint4(0u, 0u, 0u, 0u);
+        if (w0 + c * RPI + lane / CH < r0 + rows) {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(base + at.tok * a.q.ld + at.rem * a.q.hs);
           qv[c].x = h[0] | static_cast<uint32_t>(h[1]) << 16, qv[c].y = h[2] | static_cast<uint32_t>(h[3]) << 16;
           qv[c].z = h[4] | static_cast<uint32_t>(h[5]) << 16, qv[c].w = h[6] | static_cast<uint32_t>(h[7]) << 16;
         }
@@ -324,6 +338,16 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
     const int id = __ldg(table + tc.page.of(kb.at(x)));
     bad |= id < 0 || id >= a.c.pages;
   }
+  // the producer's blocks of the first step, looked up under the barrier
+  const int pblk = lane & (per - 1), patom = lane >> (C::LOG_KEYS - tc.shift);
+  auto row_of = [&](int j) -> int {  // pool row of the lane's block in step j; past the last: outside the pool, zeros
+    const int x = j * per + pblk;
+    if (patom >= D / 64 || x >= kb.n) return tc.pool_rows;
+    const int b = kb.at(x);
+    const unsigned pg = tc.page.of(b);
+    return (__ldg(table + pg) * a.c.kv_heads + kvh) * a.c.page_size + ((b - static_cast<int>(pg * tc.page.d)) << tc.shift);
+  };
+  const int row_first = BITS == 16 && warp == 8 ? row_of(0) : 0;
   const bool good = __syncthreads_or(bad) == 0;
   tc_fence_after();
   const uint32_t tmem = *slot;
@@ -337,21 +361,13 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
     }
    } else if (BITS == 16 && warp == 8) {
     // ---- producer: lane = block (and 64-dim column block) of a step ----
-    const int blk = lane & (per - 1), atom = lane >> (C::LOG_KEYS - tc.shift);
+    const int blk = pblk, atom = patom;
     const bool mine = atom < D / 64;
     const int size = 1 << tc.shift, first = kv_first(a, t0 < 0 ? 0 : t0);
     const uint32_t off = atom * C::ATOM + blk * (size * 128);
     bool ok = true;
     uint32_t raw_phase = 0;
-    // the pool row of the lane's block in step j; past the last block: outside the pool, which loads zeros
-    auto row_of = [&](int j) -> int {
-      const int x = j * per + blk;
-      if (!mine || x >= kb.n) return tc.pool_rows;
-      const int b = kb.at(x);
-      const unsigned pg = tc.page.of(b);
-      return (__ldg(table + pg) * a.c.kv_heads + kvh) * a.c.page_size + ((b - static_cast<int>(pg * tc.page.d)) << tc.shift);
-    };
-    int row = row_of(0);
+    int row = row_first;
     for (int j = 0; j < steps && ok; ++j) {
       const int st = j % C::STAGES;
       const uint32_t ph = (j / C::STAGES) & 1;
@@ -485,7 +501,7 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
       uint8_t* qs = smem + C::Q_OFF + i * C::Q_TILE;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        const int row = wrow + c * (32 / CH) + lane / CH, ch = lane % CH;
+        const int row = wrow + c * RPI + lane / CH;
         uint4 u = qv[c];
         if constexpr (BITS == 4) {
           // FP16, divided by the power of two of the row's largest element (BF16's range does not matter then), in the
@@ -677,7 +693,11 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
             const int c0 = BITS == 16 ? e : (e & ~7) + (e & 4 ? 1 : 0) + (e & 2 ? 4 : 0), c1 = BITS == 16 ? e + 1 : c0 + 2;
             const float v0 = __uint_as_float(o[c0]) * inv, v1 = __uint_as_float(o[c1]) * inv;
             nan |= v0 != v0 || v1 != v1;
-            pk[e >> 1] = kv_pack<T>(v0, v1);
+            // FP16 saturates; a row with a NaN is computed again below
+            if constexpr (std::is_same<T, __half>::value)
+              pk[e >> 1] = pack_p<T>(fminf(fmaxf(v0, -65504.0f), 65504.0f), fminf(fmaxf(v1, -65504.0f), 65504.0f));
+            else
+              pk[e >> 1] = pack_p<T>(v0, v1);
           }
 #pragma unroll
           for (int u = 0; u < 4; ++u)
@@ -685,20 +705,22 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
                 make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
         }
         __syncwarp();
+        {
+          RowWalk at(w0 + lane / CH, RPI, group);
+          T* base = static_cast<T*>(a.out.p) + sq.row0 * a.out.ld + kvh * group * a.out.hs + 8 * ch;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          const int row = c * (32 / CH) + lane / CH, ch = lane % CH, r = w0 + row;
-          if (r > w1) continue;
-          const uint4 v = *reinterpret_cast<const uint4*>(qs + (ch >> 3) * C::Q_ATOM + sw128(wrow + row, 8 * (ch & 7)));
-          const int tok = r / group;
-          T* op = static_cast<T*>(a.out.p) + (static_cast<long long>(sq.row0) + tok) * a.out.ld +
-                  (kvh * group + r - tok * group) * a.out.hs + 8 * ch;
-          if (tc.vec_o) {
-            *reinterpret_cast<uint4*>(op) = v;
-          } else {
-            uint16_t* h = reinterpret_cast<uint16_t*>(op);
-            h[0] = v.x & 0xFFFFu, h[1] = v.x >> 16, h[2] = v.y & 0xFFFFu, h[3] = v.y >> 16;
-            h[4] = v.z & 0xFFFFu, h[5] = v.z >> 16, h[6] = v.w & 0xFFFFu, h[7] = v.w >> 16;
+          for (int c = 0; c < CH; ++c, at.next()) {
+            const int row = c * RPI + lane / CH;
+            const uint4 v = *reinterpret_cast<const uint4*>(qs + (ch >> 3) * C::Q_ATOM + sw128(wrow + row, 8 * (ch & 7)));
+            T* op = base + at.tok * a.out.ld + at.rem * a.out.hs;
+            if (w0 + row > w1) continue;
+            if (tc.vec_o) {
+              *reinterpret_cast<uint4*>(op) = v;
+            } else {
+              uint16_t* h = reinterpret_cast<uint16_t*>(op);
+              h[0] = v.x & 0xFFFFu, h[1] = v.x >> 16, h[2] = v.y & 0xFFFFu, h[3] = v.y >> 16;
+              h[4] = v.z & 0xFFFFu, h[5] = v.z >> 16, h[6] = v.w & 0xFFFFu, h[7] = v.w >> 16;
+            }
           }
         }
         uint32_t redo = __ballot_sync(0xffffffffu, mine && nan);

@@ -232,7 +232,9 @@ class PagedCache:
             rq = self._rows(q, "q", None, n, dt)
             if q_out is None:
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            ro = self._rows(q_out, "q_out", heads, n, dt)
+                ro = ctypes.byref(_Rows(q_out.data_ptr(), heads * self.head_dim, self.head_dim))
+            else:
+                ro = self._rows(q_out, "q_out", heads, n, dt)
         elif q_out is not None:
             raise ValueError("q_out without q")
         rows, table = 0, None
@@ -263,7 +265,9 @@ class PagedCache:
         n, heads, dim = q.shape
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        ro = self._rows(out, "out", heads, n, q.dtype)
+            ro = ctypes.byref(_Rows(out.data_ptr(), heads * dim, dim))
+        else:
+            ro = self._rows(out, "out", heads, n, q.dtype)
         c_step = step._c(n)
         lib = _lib.lib()
         key = (n, heads, window, sinks, step.sequences, step.max_new, step.max_length, p)
