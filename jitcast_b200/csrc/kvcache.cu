@@ -61,18 +61,14 @@ __device__ __forceinline__ void store8(const KvRows& r, long long token, int hea
   }
 }
 
-// The larger (smaller) of two values, NaN if either is one: a group with a NaN has no 4-bit form and reads as NaN.
-__device__ __forceinline__ float max_nan(float a, float b) { return a != a || a > b ? a : b; }
-__device__ __forceinline__ float min_nan(float a, float b) { return a != a || a < b ? a : b; }
-
 // 8 of a group's 32 values, the rest in the 3 lanes beside this one: their codes, and the group's (scale, min).
 // scale = fp16((max − min) / 15), min = fp16(min); a code is the nearest of the 16 steps of these rounded two,
-// in FP32 with one rounding an operation, so that a value's code does not depend on where it is computed.
+// in FP32. A group with a NaN has no 4-bit form: its scale and minimum are NaN, and it reads as NaN.
 // Values beyond ±65504 (and infinities) saturate first, as 16-bit stores do; where the rounded scale would then take
 // the top code past FP16's range, a smaller one is used: 15 · scale ≤ max − min − 32, and min is off by at most 16.
 __device__ __forceinline__ uint32_t quantise8(float (&x)[8], __half2& sm) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = x[i] > 65504.0f ? 65504.0f : x[i] < -65504.0f ? -65504.0f : x[i];
+  for (int i = 0; i < 8; ++i) x[i] = max_nan(min_nan(x[i], 65504.0f), -65504.0f);
   float lo = x[0], hi = x[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) {

@@ -69,11 +69,30 @@ __device__ __forceinline__ float2 kv_unpack(uint32_t u) {
     return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u));
 }
 
+// Two values as kv_round does one: rounded to infinity past the range, which the two-wide minimum and maximum (keeping
+// NaN) bring back to ±65504.
 template <typename T>
 __device__ __forceinline__ uint32_t kv_pack(float a, float b) {
-  const T lo = kv_round<T>(a), hi = kv_round<T>(b);
-  return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&lo)) |
-         static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&hi)) << 16;
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 most = __half2half2(__ushort_as_half(0x7BFF)), least = __half2half2(__ushort_as_half(0xFBFF));
+    const __half2 h = __hmax2_nan(__hmin2_nan(__floats2half2_rn(a, b), most), least);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// The smaller (larger) of two values, NaN if either is one.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 // The value that 4-bit code c stands for: fp16(c · scale + min), one rounding (c is exact in FP16).
