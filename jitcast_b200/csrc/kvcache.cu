@@ -3,7 +3,7 @@
 // Both move each byte once and compute a few operations on it: HBM bounds them at the largest sizes, the chain
 // start → length → page table → data at the smallest. A block takes a few tokens where there are many: its warps find
 // their places in the batch side by side, then all threads move the data (one token a block left every block waiting
-// for that chain: 7 prompts 59 us, now 51; 37 chunks into 4 bits and back 170 us, now 104). A thread takes 16 dims
+// for that chain: 7 prompts 59 us, now 50; 37 chunks into 4 bits and back 170 us, now 75). A thread takes 16 dims
 // of a head: 8 in each half, so it holds whole rotation pairs, reads and writes 16-byte vectors, and 4 neighbouring
 // threads hold one 32-dim group of a 4-bit row in each half.
 #include "kernels.cuh"
@@ -140,7 +140,7 @@ __device__ __forceinline__ void find_places(const KvCache& c, const KvStep& st, 
 }
 
 template <typename T, int BITS, int D, bool VEC>
-__global__ void __launch_bounds__(512) kv_append_kernel(const __grid_constant__ KvAppendArgs a, int per_block) {
+__global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ KvAppendArgs a, int per_block) {
   constexpr int TPH = D / 16;  // threads per head
   __shared__ Place places[kTokens];
   const int row0 = blockIdx.x * per_block, n = min(per_block, a.st.tokens - row0);
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(512) kv_append_kernel(const __grid_constant__ 
 // Cached tokens as packed rows of 16-bit values (a 4-bit cache: FP16, the values its codes stand for). A thread takes
 // 8 dims.
 template <typename T, int BITS, int D, bool VEC>
-__global__ void __launch_bounds__(512) kv_read_kernel(const __grid_constant__ KvReadArgs a, int per_block) {
+__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvReadArgs a, int per_block) {
   constexpr int TPH = D / 8;
   __shared__ Place places[kTokens];
   const int row0 = blockIdx.x * per_block, n = min(per_block, a.st.tokens - row0);
@@ -272,13 +272,14 @@ bool vec_rows(const KvRows& r) {
   return r.p == nullptr || ((reinterpret_cast<uintptr_t>(r.p) & 15) == 0 && r.ld % 8 == 0 && r.hs % 8 == 0);
 }
 
-// Threads for one token's work (up to 512, in rounds of alike size), blocks over it where a token alone has more than
+// Threads for one token's work (up to 256, in rounds of alike size: blocks of 384 leave an SM a third of its threads, 59
+// against 48 us at 8016 tokens of 48 heads of 128), blocks over it where a token alone has more than
 // four rounds, and tokens a block: one while that leaves an SM fewer than eight blocks, else up to kTokens.
 struct Launch {
   dim3 grid;
   int threads, per_block;
   Launch(int tokens, int work) {
-    const int rounds = (work + 511) / 512;
+    const int rounds = (work + 255) / 256;
     threads = ((work + rounds - 1) / rounds + 31) & ~31;
     per_block = tokens / (148 * 8);
     per_block = per_block < 1 ? 1 : per_block > kTokens ? kTokens : per_block;
