@@ -86,14 +86,16 @@ __device__ __forceinline__ uint32_t quantise8(float (&x)[8], __half2& sm) {
   if (fmaf(15.0f, __half2float(scale), __half2float(low)) >= 65520.0f)
     scale = __float2half_rd(__fdiv_rd(__fsub_rd(range, 32.0f), 15.0f));
   sm = __halves2half2(scale, low);
-  // (x − min) / scale to the nearest integer: times the rounded reciprocal (off by an ulp of the quotient), clamped,
-  // and rounded by adding 2^23, which leaves the integer in the last bits. A scale of 0 gives code 0.
-  const float s = __half2float(scale), m = __half2float(low), inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
+  // (x − min) / scale to the nearest integer, ties to even. The quotient has to be the rounded one (16-bit inputs give
+  // exact ties, of which a product with the reciprocal alone breaks some: 0.04 % of the codes), which fused arithmetic
+  // gives from the rounded reciprocal r and q = d r as q + r (d − s q) (Markstein, 1990); a division each took 24 of 72 us.
+  // Then clamped, and rounded by adding 2^23, which leaves the integer in the last bits. A scale of 0 gives code 0.
+  const float s = __half2float(scale), m = __half2float(low), r = s > 0.0f ? __frcp_rn(s) : 0.0f;
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float c = fminf(fmaxf((x[i] - m) * inv, 0.0f), 15.0f) + 8388608.0f;
-    w |= (__float_as_uint(c) & 15u) << (4 * i);
+    const float d = __fsub_rn(x[i], m), q0 = __fmul_rn(d, r), q = fmaf(fmaf(-q0, s, d), r, q0);
+    w |= (__float_as_uint(fminf(fmaxf(q, 0.0f), 15.0f) + 8388608.0f) & 15u) << (4 * i);
   }
   return w;
 }

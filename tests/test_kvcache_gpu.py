@@ -422,6 +422,25 @@ def test_append_positions_in_place_and_unaligned(torch, kvcache, bits):
         assert float((v.cpu().double() - values(torch, codes, sc)).abs().max()) <= 0.3
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_four_bit_codes_are_the_nearest(torch, kvcache, dim, dtype):
+    # values on a 16-bit grid lie half way between two codes now and then: ties go to the even code, as in 64 bits. The
+    # differences from the minimum are exact in FP32, and their quotient by the scale rounds to a tie only if it is one
+    # (a quotient of two such numbers that is not a tie is further from it than FP32's rounding).
+    w = World(torch, kvcache, 4, dtype, dim, 3, 32, [900], [900])
+    g = torch.Generator().manual_seed(13)
+    x = (torch.randn((900, 3, dim), generator=g) * 2).to(w.dt)
+    w.cache.append(w.step(), x.cuda(), x.cuda())
+    sync()
+    at = torch.arange(900)
+    page = w.table[0, at // 32].long()
+    codes, scales = quantise(torch, x)
+    for pool, sc in zip(w.pools, w.scales):
+        assert torch.equal(sc.cpu()[page, :, at % 32], scales)
+        assert torch.equal(pool.cpu()[page, :, at % 32], codes)
+
+
 def test_four_bit_edges(torch, kvcache):
     # constant groups, zeros, subnormal ranges, values past FP16's range, infinities and a NaN
     x = torch.zeros((1, 1, 64), dtype=torch.bfloat16)
