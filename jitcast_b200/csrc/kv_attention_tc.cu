@@ -18,6 +18,7 @@
 // every P·V up to j and no product is touching it: the rare rescaling of O (where the running maximum moves by much)
 // needs no barrier of its own.
 #include <algorithm>
+#include <atomic>
 
 #include "gemm.h"
 #include "kv_attention.cuh"
@@ -353,146 +354,146 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
   const uint32_t tmem = *slot;
 
   if (good && warp >= 8) {
-   if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
-   if (BITS == 4 && warp != 9) {
-    if constexpr (BITS == 4) {
-      unpack_tiles<D, C>(a, tc, kb, table, kvh, steps, t0 < 0 ? 0 : t0, t1, smem, k_full, k_free, v_full, v_free, abort_flag,
-                         warp == 8 ? 0 : warp - 9, lane);
-    }
-   } else if (BITS == 16 && warp == 8) {
-    // ---- producer: lane = block (and 64-dim column block) of a step ----
-    const int blk = pblk, atom = patom;
-    const bool mine = atom < D / 64;
-    const int size = 1 << tc.shift, first = kv_first(a, t0 < 0 ? 0 : t0);
-    const uint32_t off = atom * C::ATOM + blk * (size * 128);
-    bool ok = true;
-    uint32_t raw_phase = 0;
-    int row = row_first;
-    for (int j = 0; j < steps && ok; ++j) {
-      const int st = j % C::STAGES;
-      const uint32_t ph = (j / C::STAGES) & 1;
-      const int next = row_of(j + 1);  // in flight during this step's waits
-      ok = bar_wait(k_free + st, ph ^ 1, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (lane == 0) mbar_arrive_expect_tx(k_full + st, C::TILE);
-      __syncwarp();
-      if (mine) tma_load_2d(smem + C::K_OFF + st * C::TILE + off, &tmK, k_full + st, 64 * atom, row);
-      ok = bar_wait(v_free + st, ph ^ 1, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      // keys of the step that no row of the CTA sees: their values, whatever they are, become zeros
-      const int x = j * per + blk, key0 = kb.at(x) << tc.shift;
-      const bool part = mine && x < kb.n && (key0 + size - 1 > t1 || (key0 < first && key0 + size > a.sinks));
-      const bool clear = __any_sync(0xffffffffu, part);
-      uint8_t* vt = smem + C::V_OFF + st * C::TILE + off;
-      uint64_t* bar = clear ? v_raw : v_full + st;
-      if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
-      __syncwarp();
-      if (mine) tma_load_2d(vt, &tmV, bar, 64 * atom, row);
-      if (clear) {
-        ok = bar_wait(v_raw, raw_phase, abort_flag);
-        raw_phase ^= 1;
+    if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
+    if (BITS == 4 && warp != 9) {
+      if constexpr (BITS == 4) {
+        unpack_tiles<D, C>(a, tc, kb, table, kvh, steps, t0 < 0 ? 0 : t0, t1, smem, k_full, k_free, v_full, v_free, abort_flag,
+                           warp == 8 ? 0 : warp - 9, lane);
+      }
+    } else if (BITS == 16 && warp == 8) {
+      // ---- producer: lane = block (and 64-dim column block) of a step ----
+      const int blk = pblk, atom = patom;
+      const bool mine = atom < D / 64;
+      const int size = 1 << tc.shift, first = kv_first(a, t0 < 0 ? 0 : t0);
+      const uint32_t off = atom * C::ATOM + blk * (size * 128);
+      bool ok = true;
+      uint32_t raw_phase = 0;
+      int row = row_first;
+      for (int j = 0; j < steps && ok; ++j) {
+        const int st = j % C::STAGES;
+        const uint32_t ph = (j / C::STAGES) & 1;
+        const int next = row_of(j + 1);  // in flight during this step's waits
+        ok = bar_wait(k_free + st, ph ^ 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        for (uint32_t left = __ballot_sync(0xffffffffu, part); left; left &= left - 1) {
-          const int from = __ffs(left) - 1;  // the whole warp clears that lane's block
-          const int k0 = __shfl_sync(0xffffffffu, key0, from);
-          uint8_t* p = smem + C::V_OFF + st * C::TILE + __shfl_sync(0xffffffffu, off, from);
-          for (int w = lane; w < size * 8; w += 32) {
-            const int key = k0 + (w >> 3);
-            if (key > t1 || (key < first && key >= a.sinks)) *reinterpret_cast<uint4*>(p + 16 * w) = make_uint4(0u, 0u, 0u, 0u);
+        if (lane == 0) mbar_arrive_expect_tx(k_full + st, C::TILE);
+        __syncwarp();
+        if (mine) tma_load_2d(smem + C::K_OFF + st * C::TILE + off, &tmK, k_full + st, 64 * atom, row);
+        ok = bar_wait(v_free + st, ph ^ 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        // keys of the step that no row of the CTA sees: their values, whatever they are, become zeros
+        const int x = j * per + blk, key0 = kb.at(x) << tc.shift;
+        const bool part = mine && x < kb.n && (key0 + size - 1 > t1 || (key0 < first && key0 + size > a.sinks));
+        const bool clear = __any_sync(0xffffffffu, part);
+        uint8_t* vt = smem + C::V_OFF + st * C::TILE + off;
+        uint64_t* bar = clear ? v_raw : v_full + st;
+        if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
+        __syncwarp();
+        if (mine) tma_load_2d(vt, &tmV, bar, 64 * atom, row);
+        if (clear) {
+          ok = bar_wait(v_raw, raw_phase, abort_flag);
+          raw_phase ^= 1;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          for (uint32_t left = __ballot_sync(0xffffffffu, part); left; left &= left - 1) {
+            const int from = __ffs(left) - 1;  // the whole warp clears that lane's block
+            const int k0 = __shfl_sync(0xffffffffu, key0, from);
+            uint8_t* p = smem + C::V_OFF + st * C::TILE + __shfl_sync(0xffffffffu, off, from);
+            for (int w = lane; w < size * 8; w += 32) {
+              const int key = k0 + (w >> 3);
+              if (key > t1 || (key < first && key >= a.sinks)) *reinterpret_cast<uint4*>(p + 16 * w) = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_full + st);
+        }
+        row = next;
+      }
+      if (!ok) {
+        if (lane == 0) {
+          *abort_flag = 1;
+          atomicOr(a.err, kErrAttnWait);
+        }
+        // the copies in flight land before the CTA's shared memory can go
+        __syncwarp();
+        for (int i = 0; i < C::STAGES; ++i) {
+          mbar_wait(k_full + i, 0, 1000000);
+          mbar_wait(v_full + i, 0, 1000000);
+        }
+      }
+    } else if (warp == 9) {
+      // ---- MMA issuer ----
+      // The whole warp runs it, one elected lane issues: what the instructions take stays in uniform registers (with one
+      // lane in a branch of its own, an MMA took 80 clocks to issue).
+      if (steps > 0) {
+        const bool leader = elect_one();
+        constexpr uint32_t fmt = std::is_same<M, __half>::value ? 0u : 1u;
+        constexpr uint32_t is = idesc_f32acc(fmt, kRows, C::KEYS);
+        constexpr uint32_t io = idesc_f32acc(fmt, kRows, D) | (1u << 16);  // B (V) MN-major
+        const uint32_t qa = smem_u32(smem + C::Q_OFF), ka = smem_u32(smem + C::K_OFF), va = smem_u32(smem + C::V_OFF);
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t ph) {
+          ok = ok && __all_sync(0xffffffffu, bar_wait(bar, ph, abort_flag));
+          return ok;
+        };
+        auto scores = [&](int i, int j) {  // S_i of step j
+          if (!leader) return;
+          const uint32_t q = qa + i * C::Q_TILE, k = ka + (j % C::STAGES) * C::TILE;
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d)
+            umma_bf16(tmem + i * C::KEYS, sdesc_k_sw128(q + (d >> 2) * C::Q_ATOM + 32 * (d & 3)),
+                      sdesc_k_sw128(k + (d >> 2) * C::ATOM + 32 * (d & 3)), is, d > 0);
+          umma_commit(s_full + i);
+        };
+        auto commit = [&](uint64_t* bar) {
+          if (leader) umma_commit(bar);
+        };
+        auto values = [&](int i, int j) {  // O_i of step j
+          if (!leader) return;
+          const uint32_t v = va + (j % C::STAGES) * C::TILE;
+#pragma unroll
+          for (int k = 0; k < C::KEYS / 16; ++k)
+            umma_f16_ts(tmem + C::O_COL + i * D, tmem + i * C::KEYS + 8 * k, sdesc_v(v + 2048 * k, C::ATOM), io,
+                        j > 0 || k > 0);
+        };
+        wait(k_full, 0);
+        for (int i = 0; i < tiles && ok; ++i) {
+          // long walks: tile 1 starts when tile 0 has its first P, and the offset stays: one tile's exponentials run
+          // under the other's products (20,000 keys, 64 dims: 288 -> 256 us)
+          if (!wait(q_full + i, 0) || (C::KEYS == 128 && i == 1 && steps > 24 && !wait(p_full, 0))) break;
+          tc_fence_after();
+          scores(i, 0);
+        }
+        if (ok) commit(k_free);
+        for (int j = 0; j < steps && ok; ++j) {
+          const int jn = j + 1;
+          if (jn < steps) wait(k_full + jn % C::STAGES, (jn / C::STAGES) & 1);
+          wait(v_full + j % C::STAGES, (j / C::STAGES) & 1);
+          for (int i = 0; i < tiles && ok; ++i) {
+            if (!wait(p_full + i, j & 1)) break;
+            tc_fence_after();
+            values(i, j);
+            if (jn < steps)
+              scores(i, jn);
+            else
+              commit(o_full + i);
+          }
+          if (ok) {
+            commit(v_free + j % C::STAGES);
+            if (jn < steps) commit(k_free + jn % C::STAGES);
           }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(v_full + st);
+        if (!ok && leader) {
+          *abort_flag = 1;
+          atomicOr(a.err, kErrAttnWait);
+          umma_commit(drain);  // every product issued has completed once this flips
+          mbar_wait(drain, 0, 1000000);
+        }
       }
-      row = next;
-    }
-    if (!ok) {
-      if (lane == 0) {
-        *abort_flag = 1;
-        atomicOr(a.err, kErrAttnWait);
-      }
-      // the copies in flight land before the CTA's shared memory can go
       __syncwarp();
-      for (int i = 0; i < C::STAGES; ++i) {
-        mbar_wait(k_full + i, 0, 1000000);
-        mbar_wait(v_full + i, 0, 1000000);
-      }
     }
-   } else if (warp == 9) {
-    // ---- MMA issuer ----
-    // The whole warp runs it, one elected lane issues: what the instructions take stays in uniform registers (with one
-    // lane in a branch of its own, an MMA took 80 clocks to issue).
-    if (steps > 0) {
-      const bool leader = elect_one();
-      constexpr uint32_t fmt = std::is_same<M, __half>::value ? 0u : 1u;
-      constexpr uint32_t is = idesc_f32acc(fmt, kRows, C::KEYS);
-      constexpr uint32_t io = idesc_f32acc(fmt, kRows, D) | (1u << 16);  // B (V) MN-major
-      const uint32_t qa = smem_u32(smem + C::Q_OFF), ka = smem_u32(smem + C::K_OFF), va = smem_u32(smem + C::V_OFF);
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t ph) {
-        ok = ok && __all_sync(0xffffffffu, bar_wait(bar, ph, abort_flag));
-        return ok;
-      };
-      auto scores = [&](int i, int j) {  // S_i of step j
-        if (!leader) return;
-        const uint32_t q = qa + i * C::Q_TILE, k = ka + (j % C::STAGES) * C::TILE;
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d)
-          umma_bf16(tmem + i * C::KEYS, sdesc_k_sw128(q + (d >> 2) * C::Q_ATOM + 32 * (d & 3)),
-                    sdesc_k_sw128(k + (d >> 2) * C::ATOM + 32 * (d & 3)), is, d > 0);
-        umma_commit(s_full + i);
-      };
-      auto commit = [&](uint64_t* bar) {
-        if (leader) umma_commit(bar);
-      };
-      auto values = [&](int i, int j) {  // O_i of step j
-        if (!leader) return;
-        const uint32_t v = va + (j % C::STAGES) * C::TILE;
-#pragma unroll
-        for (int k = 0; k < C::KEYS / 16; ++k)
-          umma_f16_ts(tmem + C::O_COL + i * D, tmem + i * C::KEYS + 8 * k, sdesc_v(v + 2048 * k, C::ATOM), io,
-                      j > 0 || k > 0);
-      };
-      wait(k_full, 0);
-      for (int i = 0; i < tiles && ok; ++i) {
-        // long walks: tile 1 starts when tile 0 has its first P, and the offset stays: one tile's exponentials run
-        // under the other's products (20,000 keys, 64 dims: 288 -> 256 us)
-        if (!wait(q_full + i, 0) || (C::KEYS == 128 && i == 1 && steps > 24 && !wait(p_full, 0))) break;
-        tc_fence_after();
-        scores(i, 0);
-      }
-      if (ok) commit(k_free);
-      for (int j = 0; j < steps && ok; ++j) {
-        const int jn = j + 1;
-        if (jn < steps) wait(k_full + jn % C::STAGES, (jn / C::STAGES) & 1);
-        wait(v_full + j % C::STAGES, (j / C::STAGES) & 1);
-        for (int i = 0; i < tiles && ok; ++i) {
-          if (!wait(p_full + i, j & 1)) break;
-          tc_fence_after();
-          values(i, j);
-          if (jn < steps)
-            scores(i, jn);
-          else
-            commit(o_full + i);
-        }
-        if (ok) {
-          commit(v_free + j % C::STAGES);
-          if (jn < steps) commit(k_free + jn % C::STAGES);
-        }
-      }
-      if (!ok && leader) {
-        *abort_flag = 1;
-        atomicOr(a.err, kErrAttnWait);
-        umma_commit(drain);  // every product issued has completed once this flips
-        mbar_wait(drain, 0, 1000000);
-      }
-    }
-    __syncwarp();
-   }
   } else if (good) {
     // ---- softmax: tile i, a thread a row ----
     if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
@@ -770,13 +771,21 @@ cudaError_t launch_tc(const KvAttnArgs& a, cudaStream_t s) {
   if (BITS == 16 && (!make_operand_map(&mk, a.c.k, op, tc.pool_rows, D, D, 1 << tc.shift) ||
                      !make_operand_map(&mv, a.c.v, op, tc.pool_rows, D, D, 1 << tc.shift)))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(kv_attention_tc_kernel<T, BITS, D, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  // once a device: its shared memory, and that the warpgroups' shares add up to the registers of the launch
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  // the warpgroups' shares add up to the launch's registers only if it has this many
-  if (C::SPLIT_REGS) {
-    cudaFuncAttributes at{};
-    if ((e = cudaFuncGetAttributes(&at, kv_attention_tc_kernel<T, BITS, D, LONG>)) != cudaSuccess) return e;
-    if (at.numRegs != C::REGS) return cudaErrorInvalidConfiguration;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kv_attention_tc_kernel<T, BITS, D, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    if (C::SPLIT_REGS) {
+      cudaFuncAttributes at{};
+      if ((e = cudaFuncGetAttributes(&at, kv_attention_tc_kernel<T, BITS, D, LONG>)) != cudaSuccess) return e;
+      if (at.numRegs != C::REGS) return cudaErrorInvalidConfiguration;
+    }
+    ready.fetch_or(bit, std::memory_order_relaxed);
   }
   const dim3 grid(static_cast<unsigned>(tc.supers) * a.c.kv_heads, a.st.sequences);
   kv_attention_tc_kernel<T, BITS, D, LONG><<<grid, C::THREADS, C::SMEM, s>>>(mk, mv, a, tc);
