@@ -1,6 +1,7 @@
 // C-ABI entry points of the paged key/value cache: append (with the position rotation), attention of new tokens
 // over it, and reading cached tokens back. Every argument that the host can see is checked before a launch; what
-// only the GPU can see (starts, lengths, page ids, positions) is held to the call's bounds by the kernels.
+// only the GPU can see (starts, lengths, page ids, positions) is held to the call's bounds by the kernels. No C++ exception
+// (an allocation of a message or a device's first use may throw) leaves an entry point.
 #include <cmath>
 #include <string>
 
@@ -89,6 +90,9 @@ jc_status check_attention(jc_precision precision, const jc_kv_cache* cache, cons
   if (jc_status st = check_step(step, &a->st)) return st;
   if (heads < 1 || heads % a->c.kv_heads != 0) return fail(JC_ERR_INVALID_ARG, "heads must be a multiple of kv_heads");
   if (heads > 65535) return fail(JC_ERR_UNSUPPORTED_SHAPE, "at most 65535 heads");
+  const long long group = heads / a->c.kv_heads;
+  if (a->st.max_new * group > (1 << 30) || a->st.max_new * group / 256 * a->c.kv_heads > (1 << 30))
+    return fail(JC_ERR_UNSUPPORTED_SHAPE, "above 2^30 query rows");
   if (window < 0 || sinks < 0) return fail(JC_ERR_INVALID_ARG, "window and sinks must be >= 0");
   a->heads = heads;
   a->window = window;
@@ -103,7 +107,7 @@ extern "C" {
 jc_status jc_kv_append_device(int device, jc_precision precision, const jc_kv_cache* cache, const jc_kv_step* step,
                               const jc_kv_rows* k, const jc_kv_rows* v, const jc_kv_rows* q, int heads,
                               const jc_kv_rows* q_out, const int32_t* positions, const float* rope_table,
-                              int rope_rows, int rope_pairs, void* stream) {
+                              int rope_rows, int rope_pairs, void* stream) try {
   clear_error();
   KvAppendArgs a{};
   if (jc_status st = check_cache(precision, cache, &a.c)) return st;
@@ -135,21 +139,25 @@ jc_status jc_kv_append_device(int device, jc_precision precision, const jc_kv_ca
   a.err = rt->err;
   const cudaError_t e = launch_kv_append(a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? JC_OK : fail_cuda(e, "cache append launch");
+} catch (...) {
+  return JC_ERR_INTERNAL;
 }
 
 jc_status jc_kv_attention_workspace(jc_precision precision, const jc_kv_cache* cache, const jc_kv_step* step,
-                                    int heads, int window, int sinks, long long* bytes) {
+                                    int heads, int window, int sinks, long long* bytes) try {
   clear_error();
   if (!bytes) return fail(JC_ERR_INVALID_ARG, "null bytes");
   KvAttnArgs a{};
   if (jc_status st = check_attention(precision, cache, step, heads, window, sinks, &a)) return st;
   *bytes = kv_attention_workspace(a);
   return JC_OK;
+} catch (...) {
+  return JC_ERR_INTERNAL;
 }
 
 jc_status jc_kv_attention_device(int device, jc_precision precision, const jc_kv_cache* cache, const jc_kv_step* step,
                                  const jc_kv_rows* q, int heads, const jc_kv_rows* out, int window, int sinks,
-                                 float scale, void* workspace, long long workspace_bytes, void* stream) {
+                                 float scale, void* workspace, long long workspace_bytes, void* stream) try {
   clear_error();
   KvAttnArgs a{};
   if (jc_status st = check_attention(precision, cache, step, heads, window, sinks, &a)) return st;
@@ -173,10 +181,12 @@ jc_status jc_kv_attention_device(int device, jc_precision precision, const jc_kv
   a.err = rt->err;
   const cudaError_t e = launch_kv_attention(a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? JC_OK : fail_cuda(e, "cache attention launch");
+} catch (...) {
+  return JC_ERR_INTERNAL;
 }
 
 jc_status jc_kv_read_device(int device, jc_precision precision, const jc_kv_cache* cache, const jc_kv_step* step,
-                            const jc_kv_rows* k, const jc_kv_rows* v, void* stream) {
+                            const jc_kv_rows* k, const jc_kv_rows* v, void* stream) try {
   clear_error();
   KvReadArgs a{};
   if (jc_status st = check_cache(precision, cache, &a.c)) return st;
@@ -193,6 +203,8 @@ jc_status jc_kv_read_device(int device, jc_precision precision, const jc_kv_cach
   a.err = rt->err;
   const cudaError_t e = launch_kv_read(a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? JC_OK : fail_cuda(e, "cache read launch");
+} catch (...) {
+  return JC_ERR_INTERNAL;
 }
 
 }  // extern "C"
