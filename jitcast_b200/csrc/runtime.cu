@@ -1,6 +1,7 @@
 // Device runtimes, scratch slots and error reporting for the C ABI.
 #include "runtime.h"
 
+#include <atomic>
 #include <memory>
 
 #include "ptx.cuh"
@@ -11,6 +12,8 @@ namespace {
 thread_local std::string t_error;
 std::mutex g_rt_mu;
 std::vector<std::unique_ptr<DeviceRt>> g_rts;
+// The runtimes made so far, read without the lock or a device count: a call's share of a microsecond.
+std::atomic<DeviceRt*> g_made[64];
 }  // namespace
 
 void set_error(const std::string& msg) { t_error = msg; }
@@ -29,6 +32,8 @@ jc_status fail_cuda(cudaError_t e, const char* what) {
 }
 
 DeviceRt* device_rt(int device, std::string* why) {
+  if (device >= 0 && device < 64)
+    if (DeviceRt* made = g_made[device].load(std::memory_order_acquire)) return made;
   int count = 0;
   if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) {
     cudaGetLastError();
@@ -56,6 +61,7 @@ DeviceRt* device_rt(int device, std::string* why) {
       return nullptr;
     }
     g_rts[device] = std::move(rt);
+    if (device < 64) g_made[device].store(g_rts[device].get(), std::memory_order_release);
   }
   return g_rts[device].get();
 }
