@@ -214,6 +214,43 @@ def test_many_token_attention(torch, kvcache, case, bits, dtype, dim):
 
 
 @pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("page", [256, 592, 1024])
+@pytest.mark.parametrize("new", [1, 40])
+def test_large_pages(torch, kvcache, bits, page, new):
+    w = World(torch, kvcache, bits, "bf16", 64, 2, page, [1300, 40, 593], [new, new, new])
+    check(torch, w, "bf16", 4, window=500, sinks=20)
+    check(torch, w, "bf16", 4)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_token_of_many_heads_a_kv_head(torch, kvcache, bits, dim):
+    # more query rows of one token than the splits take: the tiles, with and without starts
+    w = World(torch, kvcache, bits, "fp16", dim, 2, 64, [300, 1, 77], [1, 1, 1])
+    a = check(torch, w, "fp16", 80, window=90, sinks=2)
+    assert torch.equal(a, check(torch, w, "fp16", 80, window=90, sinks=2, start=False))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_many_sequences(torch, kvcache, bits):
+    # hundreds of sequences, some without new tokens, some without any: every token finds its own
+    lengths = [(7 * s) % 50 for s in range(333)]
+    news = [min(n, (3 * s) % 4) for s, n in enumerate(lengths)]
+    w = World(torch, kvcache, bits, "bf16", 64, 1, 16, lengths, news)
+    check(torch, w, "bf16", 2)
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn((w.tokens, 1, 64), generator=g).to(w.dt).cuda()
+    w.cache.append(w.step(), x, x)
+    k, v = w.cache.read(w.step(), w.tokens)
+    sync()
+    if bits == 16:
+        assert torch.equal(k, x) and torch.equal(v, x)
+    else:
+        codes, sc = quantise(torch, x.cpu())
+        assert torch.equal(k.cpu().double(), values(torch, codes, sc)) and torch.equal(k, v)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("new", [1, 2, 5, 70])
 def test_long_histories(torch, kvcache, bits, new):
     # key ranges split over many blocks and joined; lengths that end inside a page and a tile
