@@ -19,6 +19,7 @@
 // needs no barrier of its own.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "gemm.h"
 #include "kv_attention.cuh"
@@ -794,9 +795,39 @@ cudaError_t launch_tc(const KvAttnArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-// Rows from which the tensor-core tiles are used: a 128-row tile costs the same for one row as for all.
+// The most keys that a row sees.
+static long long most_keys(const KvAttnArgs& a) {
+  return a.window > 0 ? std::min<long long>(a.st.max_length, static_cast<long long>(a.window) + a.sinks) : a.st.max_length;
+}
+
+static long long tile_ctas(const KvAttnArgs& a) {
+  const long long rows = static_cast<long long>(a.st.max_new) * (a.heads / a.c.kv_heads);
+  return (rows + 2 * kRows - 1) / (2 * kRows) * a.c.kv_heads * a.st.sequences;
+}
+
+// Two CTAs an SM where there are that many, or where a walk is a few steps (64 sequences of 130 tokens: 47 against
+// 78 us; 64 of 1000: 394 against 530 us; 36 of 256 new tokens over 4096: alike); one with longer steps where there are
+// not (9 of 256 over 20,000, 144 CTAs: 256 against 454 us).
+static bool short_tiles(const KvAttnArgs& a) {
+  return a.c.bits == 16 && a.c.dim == 64 && (tile_ctas(a) >= 2 * 148 || most_keys(a) <= 512);
+}
+
+// Tiles or splits. A 256-row tile walks all of its keys in one CTA, however few rows it has; splits spread the keys over
+// the GPU but read them once every 16 rows. Up to 32 rows go to the splits; above, the smaller of two estimates in
+// microseconds, from calls of 40 to 1024 rows, 500 to 20,000 keys and 1 to 1024 kv heads x sequences: tiles take 128 keys
+// a wave of CTAs in 1.55 (64 dims), 1.85 (128 dims), 2.6 (64 dims, two CTAs an SM), over 4 bits 2.5 and 3.5; splits take
+// 3 ps (128 dims: 5) a row and key. 8 kv heads, 20,000 keys: 40 rows 231 by tiles and 31 by splits (64 dims), 256 rows
+// 297 and 209, 1024 rows 298 and 650 (128 dims); 64 x 8 kv heads, 40 rows, 4000 keys: 252 and 461.
 bool kv_attention_tc_ok(const KvAttnArgs& a) {
-  return static_cast<long long>(a.st.max_new) * (a.heads / a.c.kv_heads) > 32;
+  const long long rows = static_cast<long long>(a.st.max_new) * (a.heads / a.c.kv_heads);
+  if (rows <= 32) return false;
+  const double keys = static_cast<double>(most_keys(a)), heads = static_cast<double>(a.c.kv_heads) * a.st.sequences;
+  const bool twice = short_tiles(a), wide = a.c.dim == 128;
+  const long long slots = twice ? 2 * 148 : 148, waves = (tile_ctas(a) + slots - 1) / slots;
+  const double step = a.c.bits == 4 ? (wide ? 3.5 : 2.5) : wide ? 1.85 : twice ? 2.6 : 1.55;
+  const double tiles = 10.0 + static_cast<double>(waves) * std::ceil(keys / 128.0) * step;
+  const double splits = 13.0 + static_cast<double>((rows + 15) / 16 * 16) * keys * heads * (wide ? 5e-6 : 3e-6);
+  return tiles <= splits;
 }
 
 cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, cudaStream_t s) {
@@ -805,14 +836,7 @@ cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, cudaStream_t s) {
     return a.c.f16 ? launch_tc<__half, 4, 64, 1>(a, s) : launch_tc<__nv_bfloat16, 4, 64, 1>(a, s);
   }
   if (a.c.dim == 128) return a.c.f16 ? launch_tc<__half, 16, 128, 1>(a, s) : launch_tc<__nv_bfloat16, 16, 128, 1>(a, s);
-  // Two CTAs an SM where there are that many, or where a walk is a few steps (64 sequences of 130 tokens: 49 against
-  // 78 us; 64 of 1000: 394 against 530 us; 36 of 256 new tokens over 4096: alike); one with longer steps where there are
-  // not (9 of 256 over 20,000, 144 CTAs: 256 against 454 us).
-  const long long keys = a.window > 0 ? std::min<long long>(a.st.max_length, static_cast<long long>(a.window) + a.sinks)
-                                      : a.st.max_length;
-  const long long rows = static_cast<long long>(a.st.max_new) * (a.heads / a.c.kv_heads);
-  const long long ctas = (rows + 2 * kRows - 1) / (2 * kRows) * a.c.kv_heads * a.st.sequences;
-  if (ctas >= 2 * 148 || keys <= 512) return a.c.f16 ? launch_tc<__half, 16, 64, 0>(a, s) : launch_tc<__nv_bfloat16, 16, 64, 0>(a, s);
+  if (short_tiles(a)) return a.c.f16 ? launch_tc<__half, 16, 64, 0>(a, s) : launch_tc<__nv_bfloat16, 16, 64, 0>(a, s);
   return a.c.f16 ? launch_tc<__half, 16, 64, 1>(a, s) : launch_tc<__nv_bfloat16, 16, 64, 1>(a, s);
 }
 

@@ -213,6 +213,18 @@ def test_many_token_attention(torch, kvcache, case, bits, dtype, dim):
     check(torch, w, dtype, heads, window, sinks)
 
 
+# The library takes few rows of few heads to one kernel and many to another: the same cases with 16 (8) times the heads.
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("i", [0, 1, 2, 3, 4, 5, 7, 9, 10])
+def test_many_token_attention_of_many_heads(torch, kvcache, i, bits, dim):
+    heads, kv, page, lengths, news, window, sinks = MANY[i]
+    f = 8 if kv >= 4 else 16
+    dtype = "bf16" if (i + bits + dim // 64) % 2 else "fp16"
+    w = World(torch, kvcache, bits, dtype, dim, kv * f, page, lengths, news)
+    check(torch, w, dtype, heads * f, window, sinks)
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("page", [256, 592, 1024])
 @pytest.mark.parametrize("new", [1, 40])
@@ -270,15 +282,37 @@ def test_peaked_scores(torch, kvcache, bits, new):
 
 
 @pytest.mark.parametrize("bits", [16, 4])
-@pytest.mark.parametrize("new", [1, 3, 150])
-def test_strides_and_alignment(torch, kvcache, bits, new):
+@pytest.mark.parametrize("dim", [64, 128])
+def test_peaked_scores_of_many_heads(torch, kvcache, bits, dim):
+    # the same where whole steps are taken against an old maximum: late keys far above the ones before
+    w = World(torch, kvcache, bits, "bf16", dim, 12, 64, [1400], [100], share=4.0)
+    for pool in (0, 1):  # keys 900 .. 931 three times as large
+        pages = w.table[0, torch.arange(900, 932) // 64].long()
+        at = torch.arange(900, 932) % 64
+        if bits == 16:
+            p = w.pools[pool].cpu()
+            p[pages, :, at] = p[pages, :, at] * 3
+            w.pools[pool].copy_(p)
+            w.held[0][pool][900:932] = p[pages, :, at].double()
+        else:
+            sc = w.scales[pool].cpu()
+            sc[pages, :, at] = sc[pages, :, at] * 3
+            w.scales[pool].copy_(sc)
+            w.held[0][pool][900:932] = values(torch, w.pools[pool].cpu()[pages, :, at], sc[pages, :, at])
+    check(torch, w, "bf16", 12, scale=0.25)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("new,kv", [(1, 2), (3, 2), (150, 2), (150, 16)])
+def test_strides_and_alignment(torch, kvcache, bits, new, kv):
     # q as a block of a wider row, then one whose rows and heads start off 16-byte boundaries; out the same way
-    w = World(torch, kvcache, bits, "bf16", 64, 2, 64, [400, 151], [new, new])
+    heads = 3 * kv
+    w = World(torch, kvcache, bits, "bf16", 64, kv, 64, [400, 151], [new, new])
     g = torch.Generator().manual_seed(5)
-    q = torch.randn((w.tokens, 6, 64), generator=g).to(w.dt)
+    q = torch.randn((w.tokens, heads, 64), generator=g).to(w.dt)
     exp = w.expect(q, 100, 2)
     for pad, off in ((64, 64), (3, 1)):
-        wide = torch.full((w.tokens, 6, 64 + pad), float("nan"), dtype=w.dt, device="cuda")
+        wide = torch.full((w.tokens, heads, 64 + pad), float("nan"), dtype=w.dt, device="cuda")
         view = wide[:, :, off:off + 64]
         view.copy_(q)
         out_wide = torch.full_like(wide, 7.0)
@@ -293,12 +327,12 @@ def test_strides_and_alignment(torch, kvcache, bits, new):
 
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("new", [1, 4, 200])
-def test_hidden_values_stay_out(torch, kvcache, bits, dim, new):
+@pytest.mark.parametrize("new,kv", [(1, 2), (4, 2), (200, 2), (200, 24)])
+def test_hidden_values_stay_out(torch, kvcache, bits, dim, new, kv):
     # NaN and infinities in keys and values that a token does not see: those after it, those that its window has left
     # behind (their whole pages gone from the table too), and none of them in its output
-    w = World(torch, kvcache, bits, "fp16", dim, 2, 64, [700], [new])
-    window, sinks = 90, 70
+    w = World(torch, kvcache, bits, "fp16", dim, kv, 64, [700], [new])
+    heads, window, sinks = 2 * kv, 90, 70
     first = 700 - new + 1 - window  # the first key that any token sees past the sinks
     for t, fill in ((w.pools, float("nan")), (w.pools, float("inf"))):
         for which in range(2):
@@ -308,7 +342,7 @@ def test_hidden_values_stay_out(torch, kvcache, bits, dim, new):
         table = w.table.clone()
         for page in range(2, first // 64):
             w.table[0, page] = -1
-        check(torch, w, "fp16", 4, window, sinks)
+        check(torch, w, "fp16", heads, window, sinks)
         w.table = table
     if new > 1:  # a NaN value of the last token reaches that token alone
         page, row = int(w.table[0, 699 // 64]), 699 % 64
@@ -317,7 +351,7 @@ def test_hidden_values_stay_out(torch, kvcache, bits, dim, new):
         else:
             w.scales[1][page, :, row, 0] = float("nan")
         g = torch.Generator().manual_seed(1)
-        q = torch.randn((w.tokens, 4, dim), generator=g).to(w.dt)
+        q = torch.randn((w.tokens, heads, dim), generator=g).to(w.dt)
         got = w.cache.attention(w.step(), q.cuda(), window=window, sinks=sinks)
         sync()
         got = got.cpu().double()
@@ -526,11 +560,11 @@ def test_large_and_small_queries(torch, kvcache, bits):
 
 
 @pytest.mark.parametrize("bits", [16, 4])
-@pytest.mark.parametrize("new", [1, 200])
-def test_streams_and_graphs(torch, kvcache, bits, new):
-    w = World(torch, kvcache, bits, "fp16", 64, 2, 64, [9000, 200], [new, new])
+@pytest.mark.parametrize("new,kv", [(1, 2), (200, 2), (200, 16)])
+def test_streams_and_graphs(torch, kvcache, bits, new, kv):
+    w = World(torch, kvcache, bits, "fp16", 64, kv, 64, [9000, 200], [new, new])
     g = torch.Generator().manual_seed(4)
-    q = torch.randn((w.tokens, 4, 64), generator=g).to(w.dt)
+    q = torch.randn((w.tokens, 2 * kv, 64), generator=g).to(w.dt)
     exp = w.cache.attention(w.step(), q.cuda())
     sync()
     side = torch.cuda.Stream()
@@ -590,6 +624,28 @@ def test_steps_outside_their_bounds_are_reported(torch, kvcache):
         w.cache.append(w.step(), q, q, rope=kvcache.rope_table(62, 64))
         sync()
     sync()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("new,kv", [(1, 2), (90, 2), (90, 32)])
+def test_a_page_outside_the_pool_is_left_out(torch, kvcache, bits, new, kv):
+    w = World(torch, kvcache, bits, "fp16", 64, kv, 32, [200, 150], [new, new])
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn((w.tokens, kv, 64), generator=g).to(w.dt)
+    exp = w.expect(q, 0, 0)
+    w.table[1, 1] = 10 ** 6
+    got = w.cache.attention(w.step(), q.cuda())
+    with pytest.raises(_lib.JcArgumentError):
+        sync()
+    assert float((got.cpu().double() - exp)[:new].abs().max()) <= bar(w, "fp16")  # the other sequence
+    held = w.held[1]
+    keep = [j for j in range(150) if not 32 <= j < 64]
+    for i in (0, new - 1):  # without the page's keys
+        at = 150 - new + i
+        j = torch.tensor([x for x in keep if x <= at])
+        z = torch.einsum("hd,jhd->hj", q[new + i].double(), held[0][j]) * 0.125
+        o = torch.einsum("hj,jhd->hd", torch.softmax(z, -1), held[1][j])
+        assert float((got[new + i].cpu().double() - o).abs().max()) <= bar(w, "fp16")
 
 
 def test_refusals(torch, kvcache):
