@@ -3,7 +3,7 @@
 // Both move each byte once and compute a few operations on it: HBM bounds them at the largest sizes, the chain
 // start → length → page table → data at the smallest. A block takes a few tokens where there are many: its warps find
 // their places in the batch side by side, then all threads move the data (one token a block left every block waiting
-// for that chain: 7 prompts 59 us, now 50; 37 chunks into 4 bits and back 170 us, now 75). A thread takes 16 dims
+// for that chain: 7 prompts 59 us, now 50; 37 chunks into 4 bits and back 170 us, now 80). A thread takes 16 dims
 // of a head: 8 in each half, so it holds whole rotation pairs, reads and writes 16-byte vectors, and 4 neighbouring
 // threads hold one 32-dim group of a 4-bit row in each half.
 #include "kernels.cuh"
