@@ -208,15 +208,6 @@ __device__ __forceinline__ Tile tile_of(const KvAttnArgs& a, const KvSeq& q, int
   return x;
 }
 
-// The partial results of split s of output row r (token · heads + head): O [splits][rows][D], then (max, sum).
-__device__ __forceinline__ float* part_o(const KvAttnArgs& a, int split, long long row, int D) {
-  return a.workspace + (split * (static_cast<long long>(a.st.tokens) * a.heads) + row) * D;
-}
-__device__ __forceinline__ float2* part_ml(const KvAttnArgs& a, int splits, int split, long long row, int D) {
-  const long long rows = static_cast<long long>(a.st.tokens) * a.heads;
-  return reinterpret_cast<float2*>(a.workspace + splits * rows * D) + split * rows + row;
-}
-
 template <typename T>
 __device__ __forceinline__ void store4(T* p, float4 v, bool vec) {
   if (vec) {
@@ -657,17 +648,12 @@ void split(const KvAttnArgs& a, const SplitShape& sh, int rpt, dim3 grid, cudaSt
 }
 
 template <typename T, int BITS, int D>
-cudaError_t attend(const KvAttnArgs& a, cudaStream_t s) {
-  const SplitShape sh = shape_of(a);
-  const int rpt = rows_per_tile(a);
-  const dim3 grid(sh.tiles * a.c.kv_heads, sh.splits, a.st.sequences);
-  if (BITS == 16 || whole_steps(a))
-    split<T, BITS, D, true>(a, sh, rpt, grid, s);
-  else
-    split<T, BITS, D, BITS == 16>(a, sh, rpt, grid, s);
-  if (sh.splits == 1) return cudaGetLastError();
-  cudaLaunchConfig_t cfg{};
+cudaError_t join(const KvAttnArgs& a, const SplitShape& sh, int rows_per_tile, cudaStream_t s) {
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
   const long long rows = static_cast<long long>(a.st.max_new) * a.heads;
+  if (rows > 2147483647LL) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows), a.st.sequences);
   cfg.blockDim = dim3(128);
   cfg.stream = s;
@@ -676,16 +662,43 @@ cudaError_t attend(const KvAttnArgs& a, cudaStream_t s) {
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv_combine_kernel<T, BITS, D>, a, sh, rpt);
+  return cudaLaunchKernelEx(&cfg, kv_combine_kernel<T, BITS, D>, a, sh, rows_per_tile);
+}
+
+template <typename T, int BITS, int D>
+cudaError_t attend(const KvAttnArgs& a, cudaStream_t s) {
+  const SplitShape sh = shape_of(a);
+  const int rpt = rows_per_tile(a);
+  const dim3 grid(sh.tiles * a.c.kv_heads, sh.splits, a.st.sequences);
+  if (BITS == 16 || whole_steps(a))
+    split<T, BITS, D, true>(a, sh, rpt, grid, s);
+  else
+    split<T, BITS, D, BITS == 16>(a, sh, rpt, grid, s);
+  if (sh.splits > 1) return join<T, BITS, D>(a, sh, rpt, s);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
 long long kv_attention_workspace(const KvAttnArgs& a) {
-  if (a.st.sequences == 0 || a.st.max_new == 0 || kv_attention_tc_ok(a)) return 0;
-  const SplitShape sh = shape_of(a);
-  if (sh.splits == 1) return 0;
-  return static_cast<long long>(sh.splits) * a.st.tokens * a.heads * (a.c.dim + 2) * 4;
+  if (a.st.sequences == 0 || a.st.max_new == 0) return 0;
+  const long long splits = kv_attention_tc_ok(a) ? kv_tile_splits(a) : shape_of(a).splits;
+  return splits > 1 ? kv_split_bytes(a, splits) : 0;
+}
+
+cudaError_t launch_kv_join(const KvAttnArgs& a, int shift, int chunk, int splits, int rows_per_tile, cudaStream_t s) {
+  SplitShape sh = shape_of(a);
+  sh.shift = shift;
+  sh.chunk = chunk;
+  sh.splits = splits;
+  if (a.c.bits == 16) {
+    if (a.c.dim == 64)
+      return a.c.f16 ? join<__half, 16, 64>(a, sh, rows_per_tile, s) : join<__nv_bfloat16, 16, 64>(a, sh, rows_per_tile, s);
+    return a.c.f16 ? join<__half, 16, 128>(a, sh, rows_per_tile, s) : join<__nv_bfloat16, 16, 128>(a, sh, rows_per_tile, s);
+  }
+  if (a.c.dim == 64)
+    return a.c.f16 ? join<__half, 4, 64>(a, sh, rows_per_tile, s) : join<__nv_bfloat16, 4, 64>(a, sh, rows_per_tile, s);
+  return a.c.f16 ? join<__half, 4, 128>(a, sh, rows_per_tile, s) : join<__nv_bfloat16, 4, 128>(a, sh, rows_per_tile, s);
 }
 
 cudaError_t launch_kv_attention(const KvAttnArgs& a, cudaStream_t s) {

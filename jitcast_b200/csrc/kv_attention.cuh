@@ -29,6 +29,23 @@ __device__ __forceinline__ KvBlocks kv_blocks(const KvAttnArgs& a, int t0, int t
   return k;
 }
 
+// Blocks x0 .. x1 − 1 of those.
+struct KvSlice {
+  int a, b, n, o;
+  __device__ __forceinline__ KvSlice(const KvBlocks& k, int x0, int x1)
+      : a(k.a > x0 ? k.a - x0 : 0), b(k.a > x0 ? k.b : k.b + x0 - k.a), n(x1 - x0), o(x0) {}
+  __device__ __forceinline__ int at(int x) const { return x < a ? x + o : x - a + b; }
+};
+
+// The partial results of split s of output row r (token · heads + head): O [splits][rows][D], then (max, sum).
+__device__ __forceinline__ float* part_o(const KvAttnArgs& a, int split, long long row, int D) {
+  return a.workspace + (split * (static_cast<long long>(a.st.tokens) * a.heads) + row) * D;
+}
+__device__ __forceinline__ float2* part_ml(const KvAttnArgs& a, int splits, int split, long long row, int D) {
+  const long long rows = static_cast<long long>(a.st.tokens) * a.heads;
+  return reinterpret_cast<float2*>(a.workspace + splits * rows * D) + split * rows + row;
+}
+
 // One row of the output by one warp, key by key on the CUDA cores in FP32 (lane l holds dims l, l + 32, ..),
 // with the running maximum and sum of the softmax. It reads visible keys alone. The tiled kernels multiply a hidden
 // key's value by a probability of 0, which is NaN for an infinite or undefined value; they hand a row that comes
@@ -103,5 +120,15 @@ struct KvDiv {
     return d <= 32 ? static_cast<unsigned>((u * m) >> 32) : u / d;
   }
 };
+
+// Joins what a kernel's splits left in the workspace: rows in tiles of rows_per_tile, at most `chunk` blocks of 2^shift
+// keys a split (a tile with no more than that wrote its rows itself).
+cudaError_t launch_kv_join(const KvAttnArgs& a, int shift, int chunk, int splits, int rows_per_tile, cudaStream_t s);
+
+// Splits of the keys that the tiles of this call take, and the workspace of any split.
+int kv_tile_splits(const KvAttnArgs& a);
+inline long long kv_split_bytes(const KvAttnArgs& a, long long splits) {
+  return splits * a.st.tokens * a.heads * (a.c.dim + 2) * 4;
+}
 
 }  // namespace jc

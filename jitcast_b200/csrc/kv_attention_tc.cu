@@ -65,6 +65,7 @@ struct TcCfg {
 struct TcArgs {
   int shift;         // 2^shift keys a block: the largest power of two, up to 64, that a page holds a whole number of
   int supers;        // 256-row tiles of the longest sequence
+  int chunk, splits; // blocks that a CTA takes at most (whole steps), CTAs along the longest sequence's keys
   int pool_rows;     // rows of the pools: a coordinate outside them
   int vec_q, vec_o;  // 16-byte vectors
   KvDiv page;        // blocks of a page
@@ -156,7 +157,7 @@ __device__ __forceinline__ uint64_t sdesc_v(uint32_t saddr, uint32_t atom_bytes)
 // Within each 8 dims the values lie in the order 0, 4, 1, 5, 2, 6, 3, 7, as they come out of a word of codes: Q is written
 // in that order too, and the output's columns are put back at the end. Keys that no row sees become zeros.
 template <int D, typename C>
-__device__ __forceinline__ void unpack_tiles(const KvAttnArgs& a, const TcArgs& tc, const KvBlocks& kb, const int* table,
+__device__ __forceinline__ void unpack_tiles(const KvAttnArgs& a, const TcArgs& tc, const KvSlice& kb, const int* table,
                                              int kvh, int steps, int t0, int t1, uint8_t* smem, uint64_t* k_full,
                                              uint64_t* k_free, uint64_t* v_full, uint64_t* v_free,
                                              volatile uint32_t* abort_flag, int part, int lane) {
@@ -267,7 +268,11 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
   if (rows <= 0) return;
   const int base_t = sq.length - sq.n;
   const int t0 = base_t + r0 / group, t1 = base_t + (r0 + rows - 1) / group;
-  const KvBlocks kb = kv_blocks(a, t0, t1, tc.shift);
+  const KvBlocks all = kv_blocks(a, t0, t1, tc.shift);
+  const int split = blockIdx.z, x0 = split * tc.chunk;
+  if (split > 0 && x0 >= all.n) return;
+  const bool whole = all.n <= tc.chunk;  // no other CTA has keys of this tile
+  const KvSlice kb(all, x0, min(all.n, x0 + tc.chunk));
   const int per = C::KEYS >> tc.shift;  // blocks of a step
   const int steps = (kb.n + per - 1) >> (C::LOG_KEYS - tc.shift);
   const int tiles = rows > kRows ? 2 : 1;
@@ -675,65 +680,85 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
         if (lane == 0) atomicOr(a.err, kErrAttnWait);
       } else if (any) {
         tc_fence_after();
-        const float inv = m == -INFINITY || l == 0.0f ? 0.0f : 1.0f / l;  // no maximum: no key seen
-        bool nan = l != l;
-        // the row's values through the tile's (consumed) Q into whole-row stores
+        if (!whole) {  // O as it stands, and the row's maximum and sum
+          const int r = w0 + lane, tok = r / group, head = kvh * group + r - tok * group;
+          const long long row = (static_cast<long long>(sq.row0) + tok) * a.heads + head;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          if (steps > 0) {
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
             tmem_ld_32x32b_x32(o_col + 32 * c, o);
             tmem_ld_wait();
-          } else {
+            if (!mine) continue;
+            float4* dst = reinterpret_cast<float4*>(part_o(a, split, row, D) + 32 * c);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0u;
-          }
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            // the columns of dims e, e + 1 (4 bits: unpacked values lie in the order 0, 4, 1, 5, 2, 6, 3, 7)
-            const int c0 = BITS == 16 ? e : (e & ~7) + (e & 4 ? 1 : 0) + (e & 2 ? 4 : 0), c1 = BITS == 16 ? e + 1 : c0 + 2;
-            const float v0 = __uint_as_float(o[c0]) * inv, v1 = __uint_as_float(o[c1]) * inv;
-            nan |= v0 != v0 || v1 != v1;
-            // FP16 saturates; a row with a NaN is computed again below
-            if constexpr (std::is_same<T, __half>::value)
-              pk[e >> 1] = pack_p<T>(fminf(fmaxf(v0, -65504.0f), 65504.0f), fminf(fmaxf(v1, -65504.0f), 65504.0f));
-            else
-              pk[e >> 1] = pack_p<T>(v0, v1);
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            *reinterpret_cast<uint4*>(qs + (c >> 1) * C::Q_ATOM + sw128(wrow + lane, 8 * (4 * (c & 1) + u))) =
-                make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
-        }
-        __syncwarp();
-        {
-          RowWalk at(w0 + lane / CH, RPI, group);
-          T* base = static_cast<T*>(a.out.p) + sq.row0 * a.out.ld + kvh * group * a.out.hs + 8 * ch;
-#pragma unroll
-          for (int c = 0; c < CH; ++c, at.next()) {
-            const int row = c * RPI + lane / CH;
-            const uint4 v = *reinterpret_cast<const uint4*>(qs + (ch >> 3) * C::Q_ATOM + sw128(wrow + row, 8 * (ch & 7)));
-            T* op = base + at.tok * a.out.ld + at.rem * a.out.hs;
-            if (w0 + row > w1) continue;
-            if (tc.vec_o) {
-              *reinterpret_cast<uint4*>(op) = v;
-            } else {
-              uint16_t* h = reinterpret_cast<uint16_t*>(op);
-              h[0] = v.x & 0xFFFFu, h[1] = v.x >> 16, h[2] = v.y & 0xFFFFu, h[3] = v.y >> 16;
-              h[4] = v.z & 0xFFFFu, h[5] = v.z >> 16, h[6] = v.w & 0xFFFFu, h[7] = v.w >> 16;
+            for (int e = 0; e < 32; e += 4) {
+              const int c0 = BITS == 16 ? e : (e & ~7) + (e & 4 ? 1 : 0), st = BITS == 16 ? 1 : 2;  // as below
+              dst[e >> 2] = make_float4(__uint_as_float(o[c0]), __uint_as_float(o[c0 + st]),
+                                        __uint_as_float(o[c0 + (BITS == 16 ? 2 : 4)]), __uint_as_float(o[c0 + (BITS == 16 ? 3 : 6)]));
             }
           }
-        }
-        uint32_t redo = __ballot_sync(0xffffffffu, mine && nan);
-        __syncwarp();
-        while (redo) {
-          const int w = __ffs(redo) - 1;
-          redo &= redo - 1;
-          const int xr = w0 + w, xt = xr / group, xh = kvh * group + xr % group;
-          const long long xg = static_cast<long long>(sq.row0) + xt;
-          kv_attend_row<T, BITS, D>(a, seq, base_t + xt, xh, static_cast<const T*>(a.q.p) + xg * a.q.ld + xh * a.q.hs,
-                                  static_cast<T*>(a.out.p) + xg * a.out.ld + xh * a.out.hs);
+          if (mine) *part_ml(a, tc.splits, split, row, D) = make_float2(m, l);
+        } else {
+          const float inv = m == -INFINITY || l == 0.0f ? 0.0f : 1.0f / l;  // no maximum: no key seen
+          bool nan = l != l;
+          // the row's values through the tile's (consumed) Q into whole-row stores
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            if (steps > 0) {
+              tmem_ld_32x32b_x32(o_col + 32 * c, o);
+              tmem_ld_wait();
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = 0u;
+            }
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              // the columns of dims e, e + 1 (4 bits: unpacked values lie in the order 0, 4, 1, 5, 2, 6, 3, 7)
+              const int c0 = BITS == 16 ? e : (e & ~7) + (e & 4 ? 1 : 0) + (e & 2 ? 4 : 0), c1 = BITS == 16 ? e + 1 : c0 + 2;
+              const float v0 = __uint_as_float(o[c0]) * inv, v1 = __uint_as_float(o[c1]) * inv;
+              nan |= v0 != v0 || v1 != v1;
+              // FP16 saturates; a row with a NaN is computed again below
+              if constexpr (std::is_same<T, __half>::value)
+                pk[e >> 1] = pack_p<T>(fminf(fmaxf(v0, -65504.0f), 65504.0f), fminf(fmaxf(v1, -65504.0f), 65504.0f));
+              else
+                pk[e >> 1] = pack_p<T>(v0, v1);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              *reinterpret_cast<uint4*>(qs + (c >> 1) * C::Q_ATOM + sw128(wrow + lane, 8 * (4 * (c & 1) + u))) =
+                  make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
+          }
+          __syncwarp();
+          {
+            RowWalk at(w0 + lane / CH, RPI, group);
+            T* base = static_cast<T*>(a.out.p) + sq.row0 * a.out.ld + kvh * group * a.out.hs + 8 * ch;
+#pragma unroll
+            for (int c = 0; c < CH; ++c, at.next()) {
+              const int row = c * RPI + lane / CH;
+              const uint4 v = *reinterpret_cast<const uint4*>(qs + (ch >> 3) * C::Q_ATOM + sw128(wrow + row, 8 * (ch & 7)));
+              T* op = base + at.tok * a.out.ld + at.rem * a.out.hs;
+              if (w0 + row > w1) continue;
+              if (tc.vec_o) {
+                *reinterpret_cast<uint4*>(op) = v;
+              } else {
+                uint16_t* h = reinterpret_cast<uint16_t*>(op);
+                h[0] = v.x & 0xFFFFu, h[1] = v.x >> 16, h[2] = v.y & 0xFFFFu, h[3] = v.y >> 16;
+                h[4] = v.z & 0xFFFFu, h[5] = v.z >> 16, h[6] = v.w & 0xFFFFu, h[7] = v.w >> 16;
+              }
+            }
+          }
+          uint32_t redo = __ballot_sync(0xffffffffu, mine && nan);
+          __syncwarp();
+          while (redo) {
+            const int w = __ffs(redo) - 1;
+            redo &= redo - 1;
+            const int xr = w0 + w, xt = xr / group, xh = kvh * group + xr % group;
+            const long long xg = static_cast<long long>(sq.row0) + xt;
+            kv_attend_row<T, BITS, D>(a, seq, base_t + xt, xh, static_cast<const T*>(a.q.p) + xg * a.q.ld + xh * a.q.hs,
+                                    static_cast<T*>(a.out.p) + xg * a.out.ld + xh * a.out.hs);
+          }
         }
       }
     }
@@ -741,6 +766,10 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
     for (int r = warp; r < rows; r += C::THREADS / 32) {
       const int xr = r0 + r, xt = xr / group, xh = kvh * group + xr % group;
       const long long xg = static_cast<long long>(sq.row0) + xt;
+      if (!whole) {  // the join recomputes a row whose sum is not a number
+        if (lane == 0) *part_ml(a, tc.splits, split, xg * a.heads + xh, D) = make_float2(0.0f, NAN);
+        continue;
+      }
       kv_attend_row<T, BITS, D>(a, seq, base_t + xt, xh, static_cast<const T*>(a.q.p) + xg * a.q.ld + xh * a.q.hs,
                               static_cast<T*>(a.out.p) + xg * a.out.ld + xh * a.out.hs);
     }
@@ -751,6 +780,14 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM);
   }
+}
+
+// The most blocks of 2^shift keys that a 256-row tile reads.
+long long most_blocks(const KvAttnArgs& a, int shift) {
+  const long long group = a.heads / a.c.kv_heads, tokens = (2 * kRows + group - 2) / group + 1, size = 1ll << shift;
+  const long long reach = a.sinks + static_cast<long long>(a.window) + tokens + 2 * (size - 1);
+  const long long keys = a.window > 0 && reach < a.st.max_length ? reach : a.st.max_length;
+  return (keys + size - 1) / size;
 }
 
 template <typename T, int BITS, int D, int LONG>
@@ -788,8 +825,14 @@ cudaError_t launch_tc(const KvAttnArgs& a, cudaStream_t s) {
     }
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  const dim3 grid(static_cast<unsigned>(tc.supers) * a.c.kv_heads, a.st.sequences);
+  const int per = C::KEYS >> tc.shift;
+  tc.splits = kv_tile_splits(a);
+  const long long blocks = most_blocks(a, tc.shift);
+  tc.chunk = static_cast<int>(((blocks + tc.splits - 1) / tc.splits + per - 1) / per * per);
+  if (tc.chunk < per) tc.chunk = per;
+  const dim3 grid(static_cast<unsigned>(tc.supers) * a.c.kv_heads, a.st.sequences, tc.splits);
   kv_attention_tc_kernel<T, BITS, D, LONG><<<grid, C::THREADS, C::SMEM, s>>>(mk, mv, a, tc);
+  if (tc.splits > 1) return launch_kv_join(a, tc.shift, tc.chunk, tc.splits, 2 * kRows, s);
   return cudaGetLastError();
 }
 
@@ -812,22 +855,37 @@ static bool short_tiles(const KvAttnArgs& a) {
   return a.c.bits == 16 && a.c.dim == 64 && (tile_ctas(a) >= 2 * 148 || most_keys(a) <= 512);
 }
 
-// Tiles or splits. A 256-row tile walks all of its keys in one CTA, however few rows it has; splits spread the keys over
-// the GPU but read them once every 16 rows. Up to 32 rows go to the splits; above, the smaller of two estimates in
-// microseconds, from calls of 40 to 1024 rows, 500 to 20,000 keys and 1 to 1024 kv heads x sequences: tiles take 128 keys
-// a wave of CTAs in 1.55 (64 dims), 1.85 (128 dims), 2.6 (64 dims, two CTAs an SM), over 4 bits 2.5 and 3.5; splits take
-// 3 ps (128 dims: 5) a row and key. 8 kv heads, 20,000 keys: 40 rows 231 by tiles and 31 by splits (64 dims), 256 rows
-// 297 and 209, 1024 rows 298 and 650 (128 dims); 64 x 8 kv heads, 40 rows, 4000 keys: 252 and 461.
+// The tiles' estimated time in microseconds with their keys in `splits` parts: 128 keys a wave of CTAs in 1.55 (64 dims),
+// 1.85 (128 dims), 2.6 (64 dims, two CTAs an SM), over 4 bits 2.5 and 3.5; 10 for the call, and for the join 8 and the parts'
+// results written and read at 2 TB/s (2 x 1000 new tokens of 32 heads in 4 parts: 352 us, in one 185).
+static double tile_time(const KvAttnArgs& a, int splits) {
+  const bool twice = short_tiles(a), wide = a.c.dim == 128;
+  const long long slots = twice ? 2 * 148 : 148, waves = (tile_ctas(a) * splits + slots - 1) / slots;
+  const double step = a.c.bits == 4 ? (wide ? 3.5 : 2.5) : wide ? 1.85 : twice ? 2.6 : 1.55;
+  const double join = splits > 1 ? 8.0 + 2e-6 / 2.0 * static_cast<double>(kv_split_bytes(a, splits)) : 0.0;
+  return 10.0 + static_cast<double>(waves) * std::ceil(static_cast<double>(most_keys(a)) / 128.0 / splits) * step + join;
+}
+
+// Parts of the keys: the fewest that the estimate likes best, each of 1024 keys at least.
+int kv_tile_splits(const KvAttnArgs& a) {
+  int best = 1;
+  if (short_tiles(a)) return best;
+  for (int s = 2; s <= 16 && most_keys(a) / s >= 1024; ++s)
+    if (tile_time(a, s) < 0.95 * tile_time(a, best)) best = s;
+  return best;
+}
+
+// Tiles or splits. A tile walks its keys for 256 rows, however few it has; splits read the keys once every 16 rows. Up to
+// 32 rows go to the splits; above, the smaller of two estimates, from calls of 40 to 1024 rows, 500 to 20,000 keys and 1 to
+// 1024 kv heads x sequences; splits take 3 ps (128 dims: 5) a row and key and 13 us. 8 kv heads, 20,000 keys, tiles in one
+// part: 40 rows 231 us by tiles and 31 by splits (64 dims), 256 rows 297 and 209, 1024 rows 298 and 650 (128 dims);
+// 64 x 8 kv heads, 40 rows, 4000 keys: 252 and 461.
 bool kv_attention_tc_ok(const KvAttnArgs& a) {
   const long long rows = static_cast<long long>(a.st.max_new) * (a.heads / a.c.kv_heads);
   if (rows <= 32) return false;
   const double keys = static_cast<double>(most_keys(a)), heads = static_cast<double>(a.c.kv_heads) * a.st.sequences;
-  const bool twice = short_tiles(a), wide = a.c.dim == 128;
-  const long long slots = twice ? 2 * 148 : 148, waves = (tile_ctas(a) + slots - 1) / slots;
-  const double step = a.c.bits == 4 ? (wide ? 3.5 : 2.5) : wide ? 1.85 : twice ? 2.6 : 1.55;
-  const double tiles = 10.0 + static_cast<double>(waves) * std::ceil(keys / 128.0) * step;
-  const double splits = 13.0 + static_cast<double>((rows + 15) / 16 * 16) * keys * heads * (wide ? 5e-6 : 3e-6);
-  return tiles <= splits;
+  const double splits = 13.0 + static_cast<double>((rows + 15) / 16 * 16) * keys * heads * (a.c.dim == 128 ? 5e-6 : 3e-6);
+  return tile_time(a, kv_tile_splits(a)) <= splits;
 }
 
 cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, cudaStream_t s) {

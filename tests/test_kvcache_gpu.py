@@ -274,6 +274,34 @@ def test_long_histories(torch, kvcache, bits, new):
 
 
 @pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [64, 48])
+def test_many_rows_over_long_histories(torch, kvcache, bits, dim, page):
+    # few tiles of rows, whose keys are split over several CTAs and joined; a short sequence beside the long one, a key
+    # that not every row sees with an undefined value, and the same bits twice
+    w = World(torch, kvcache, bits, "bf16", dim, 8, page, [4500, 200], [70, 45])
+    a = check(torch, w, "bf16", 8)
+    assert torch.equal(a, check(torch, w, "bf16", 8))
+    check(torch, w, "bf16", 8, window=3300, sinks=100)
+    where, row = int(w.table[0, 4490 // page]), 4490 % page
+    if bits == 16:
+        w.pools[1][where, :, row, 5] = float("inf")
+    else:
+        w.scales[1][where, :, row, 0] = float("nan")
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn((w.tokens, 8, dim), generator=g).to(w.dt)
+    got = w.cache.attention(w.step(), q.cuda()).cpu().double()
+    sync()
+    assert float((got[:60] - a[:60]).abs().max()) <= 2 * bar(w, "bf16")  # tokens before it
+    assert not bool(got[60:70, :, 5].isfinite().any())
+    w.table[0, 20] = -7  # and a page outside the pool: reported, its keys left out
+    got = w.cache.attention(w.step(), q.cuda()).cpu().double()
+    with pytest.raises(_lib.JcArgumentError):
+        sync()
+    assert bool(got[:60].isfinite().all())
+
+
+@pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("new", [1, 40, 300])
 def test_peaked_scores(torch, kvcache, bits, new):
     # scores over a wide range: the running maximum moves often and late
