@@ -78,7 +78,7 @@ __device__ __noinline__ void kv_attend_row(const KvAttnArgs& a, int s, int t, in
     for (int w = 16; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
     const float mn = fmaxf(m, d);
     const float up = mn == -INFINITY ? 1.0f : __expf(m - mn);  // −inf − −inf would be NaN
-    const float p = mn == -INFINITY ? 0.0f : d != d ? d : __expf(d - mn);
+    const float p = d != d ? d : mn == -INFINITY ? 0.0f : __expf(d - mn);  // an undefined score stays, whatever came before
     l = l * up + p;
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = o[i] * up + p * kv_value<T, BITS>(a.c.v, a.c.v_scale, row, D, lane + 32 * i);

@@ -1,0 +1,98 @@
+"""The paged cache's attention where its arithmetic or its arguments are at an edge, against the definition in 64 bits.
+
+The bars are those of test_kvcache_gpu.py, whose cache of known contents these tests share.
+"""
+
+import math
+
+import pytest
+from test_kvcache_gpu import ROUNDING, World, bar, dtype_of, quantise, sync, values
+
+from jitcast_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    return pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def kvcache(jc):
+    from jitcast_b200 import kvcache
+
+    return kvcache
+
+
+def put(torch, w, which, s, j, x):
+    """Key (which 0) or value (1) of index j of sequence s becomes x [kv_heads, dim]: in the pools and in what they hold."""
+    x = x.to(w.dt)
+    page, row = int(w.table[s, j // w.page]), j % w.page
+    if w.bits == 16:
+        w.pools[which][page, :, row] = x.cuda()
+        w.held[s][which][j] = x.double()
+    else:
+        codes, scales = quantise(torch, x)
+        w.pools[which][page, :, row] = codes.cuda()
+        w.scales[which][page, :, row] = scales.cuda()
+        w.held[s][which][j] = values(torch, codes, scales)
+
+
+def spoil(w, which, s, j, value=float("nan"), dim=5):
+    """One dim (4 bits: its group of 32, which then reads as NaN) of index j becomes `value`."""
+    page, row = int(w.table[s, j // w.page]), j % w.page
+    if w.bits == 16:
+        w.pools[which][page, :, row, dim] = value
+        w.held[s][which][j, :, dim] = value
+    else:
+        w.scales[which][page, :, row, dim // 32] = float("nan")
+        w.held[s][which][j, :, dim // 32 * 32:dim // 32 * 32 + 32] = float("nan")
+
+
+def queries(torch, w, heads, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn((w.tokens, heads, w.dim), generator=g).to(w.dt)
+
+
+def agree(got, exp, most):
+    """NaN exactly where the definition has one, the rest within the bar."""
+    got = got.cpu().double()
+    assert bool((got.isnan() == exp.isnan()).all())
+    there = ~exp.isnan()
+    assert not there.any() or float((got - exp)[there].abs().max()) <= most
+
+
+# The forms that a call can take: (kv heads, lengths, new tokens). Whole rows by one block of the splits, rows joined from
+# several, 256-row tiles, and tiles whose keys are split over CTAs and joined.
+FORMS = {
+    "splits": (2, [90, 1, 40], [2, 1, 1]),
+    "joined splits": (2, [9000, 1, 40], [2, 1, 1]),
+    "tiles": (8, [300, 1, 40], [150, 1, 3]),
+    "joined tiles": (8, [4500, 1, 200], [70, 1, 45]),
+}
+
+
+@pytest.mark.parametrize("bits,dtype", [(16, "bf16"), (16, "fp16"), (4, "bf16")])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+def test_visible_nans_reach_the_output(torch, kvcache, form, dim, bits, dtype):
+    # a NaN score makes its row's softmax NaN, wherever the key lies and whatever came before it
+    kv, lengths, news = FORMS[form]
+    heads = 2 * kv
+    for what in ("query", "first key", "every key", "sink"):
+        w = World(torch, kvcache, bits, dtype, dim, kv, 64, lengths, news)
+        q = queries(torch, w, heads)
+        window, sinks = (20, 3) if what == "sink" else (0, 0)
+        if what == "query":
+            q[0, 1, 7] = float("nan")
+            q[w.bounds[1], heads - 1, 0] = float("nan")  # the sequence of one key
+        elif what == "every key":
+            for j in range(lengths[2]):
+                spoil(w, 0, 2, j)
+            spoil(w, 0, 1, 0)
+        else:
+            spoil(w, 0, 0, 0)
+        got = w.cache.attention(w.step(), q.cuda(), window=window, sinks=sinks)
+        sync()
+        agree(got, w.expect(q, window, sinks), bar(w, dtype))
