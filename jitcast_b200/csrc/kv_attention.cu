@@ -504,7 +504,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 2 : BITS == 4 ? 4 : 3) 
     if (whole) {
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-      if (acc.x != acc.x || acc.y != acc.y || acc.z != acc.z || acc.w != acc.w) atomicOr(&s_nan, 1u << r);
+      const bool none = sum == 0.0f && sq.length - sq.n + rr / group >= 0;  // a token of an index sees its own key at least
+      if (none || acc.x != acc.x || acc.y != acc.y || acc.z != acc.z || acc.w != acc.w) atomicOr(&s_nan, 1u << r);
       store4(static_cast<T*>(a.out.p) + row * a.out.ld + head * a.out.hs + d, acc, sh.vec_o);
     } else {
       *reinterpret_cast<float4*>(part_o(a, split, row * a.heads + head, D) + d) = acc;
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-    bad = acc.x != acc.x || acc.y != acc.y || acc.z != acc.z || acc.w != acc.w;
+    bad = (sum == 0.0f && sq.length - sq.n + i >= 0) || acc.x != acc.x || acc.y != acc.y || acc.z != acc.z || acc.w != acc.w;
     store4(static_cast<T*>(a.out.p) + (static_cast<long long>(sq.row0) + i) * a.out.ld + head * a.out.hs + 4 * d, acc, sh.vec_o);
   }
   if (__syncthreads_or(bad) && warp == 0) {

@@ -49,7 +49,8 @@ __device__ __forceinline__ float2* part_ml(const KvAttnArgs& a, int splits, int 
 // One row of the output by one warp, key by key on the CUDA cores in FP32 (lane l holds dims l, l + 32, ..),
 // with the running maximum and sum of the softmax. It reads visible keys alone. The tiled kernels multiply a hidden
 // key's value by a probability of 0, which is NaN for an infinite or undefined value; they hand a row that comes
-// out with a NaN to this form, so hidden values stay out of every result and a visible NaN stays in it.
+// out with a NaN to this form, so hidden values stay out of every result and a visible NaN stays in it. So do they with
+// a row whose sum is 0: no key of it was there (zeros), or every score is -inf (NaN, as 0 / 0 is).
 template <typename T, int BITS, int D>
 __device__ __noinline__ void kv_attend_row(const KvAttnArgs& a, int s, int t, int head, const T* q, T* out) {
   constexpr int N = D / 32;
@@ -63,6 +64,7 @@ __device__ __noinline__ void kv_attend_row(const KvAttnArgs& a, int s, int t, in
     o[i] = 0.0f;
   }
   float m = -INFINITY, l = 0.0f;
+  bool seen = false;
   const int first = kv_first(a, t), sink = a.sinks < first ? a.sinks : first;
   for (int j = sink > 0 ? 0 : first; j <= t; j = j + 1 == sink ? first : j + 1) {
     const long long page = kv_page_row(a.c, table, j / a.c.page_size, kvh);
@@ -70,6 +72,7 @@ __device__ __noinline__ void kv_attend_row(const KvAttnArgs& a, int s, int t, in
       if (lane == 0) atomicOr(a.err, kErrKvStep);
       continue;
     }
+    seen = true;
     const long long row = page + j % a.c.page_size;
     float d = 0.0f;
 #pragma unroll
@@ -84,7 +87,7 @@ __device__ __noinline__ void kv_attend_row(const KvAttnArgs& a, int s, int t, in
     for (int i = 0; i < N; ++i) o[i] = o[i] * up + p * kv_value<T, BITS>(a.c.v, a.c.v_scale, row, D, lane + 32 * i);
     m = mn;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = l != 0.0f ? 1.0f / l : seen ? NAN : 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) out[lane + 32 * i] = kv_round<T>(o[i] * inv);
 }

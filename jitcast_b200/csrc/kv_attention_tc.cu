@@ -700,7 +700,7 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
           if (mine) *part_ml(a, tc.splits, split, row, D) = make_float2(m, l);
         } else {
           const float inv = m == -INFINITY || l == 0.0f ? 0.0f : 1.0f / l;  // no maximum: no key seen
-          bool nan = l != l;
+          bool nan = l != l || (inv == 0.0f && t >= 0);  // undefined, or a token of an index that has seen no key
           // the row's values through the tile's (consumed) Q into whole-row stores
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {

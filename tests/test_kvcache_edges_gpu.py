@@ -96,3 +96,23 @@ def test_visible_nans_reach_the_output(torch, kvcache, form, dim, bits, dtype):
         got = w.cache.attention(w.step(), q.cuda(), window=window, sinks=sinks)
         sync()
         agree(got, w.expect(q, window, sinks), bar(w, dtype))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+def test_rows_of_infinitely_small_scores(torch, kvcache, form, dim, dtype):
+    # every visible score -inf: the softmax is undefined (zeros are for a token that sees no key); some: they weigh nothing
+    kv, lengths, news = FORMS[form]
+    w = World(torch, kvcache, 16, dtype, dim, kv, 64, lengths, news)
+    q = queries(torch, w, 2 * kv)
+    q[:, :, 5] = q[:, :, 5].abs() + 1
+    for j in range(lengths[2]):
+        spoil(w, 0, 2, j, float("-inf"))
+    spoil(w, 0, 1, 0, float("-inf"))
+    spoil(w, 0, 0, 0, float("-inf"))
+    got = w.cache.attention(w.step(), q.cuda())
+    sync()
+    exp = w.expect(q, 0, 0)
+    assert exp[w.bounds[1]:].isnan().all() and not exp[:w.bounds[1]].isnan().any()
+    agree(got, exp, bar(w, dtype))
