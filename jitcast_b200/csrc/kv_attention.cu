@@ -36,7 +36,7 @@ constexpr int kWarps = 4;
 constexpr int kCtasOne = 148 * 4, kCtasMany = 148 * 16, kMaxSplits = kCtasMany;
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's running maximum moves only when a score passes it by this much (as a power of two): probabilities then
-// reach 2^8, which costs no precision in any of the types, and most blocks rescale nothing.
+// reach 2^8 (FP16: 2^15, see kProbUp), which costs no precision in any of the types, and most blocks rescale nothing.
 constexpr float kLazy = 8.0f;
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 2 : BITS == 4 ? 4 : 3) 
         float p[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float base = m[i][e & 1] == -INFINITY ? 0.0f : m[i][e & 1];
+          const float base = (m[i][e & 1] == -INFINITY ? 0.0f : m[i][e & 1]) - kProbUp<M>;
           p[e] = kv_ex2(fmaf(s[u][i][e], sl2[i][e & 1], -base));
           l[i][e & 1] += p[e];
         }

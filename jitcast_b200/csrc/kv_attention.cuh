@@ -112,6 +112,12 @@ __device__ __forceinline__ float kv_ex2(float x) {
   return y;
 }
 
+// Probabilities that go into a product as FP16 are taken 2^7 times as large, and their sums with them: one below 2^-25
+// rounds to 0 in FP16, and 131,000 keys just under that beside one large one are 1/250 of a row's weight. So the bound is
+// 2^-32, 1/30,000 of it. With a maximum that lags by 2^8 at most they stay below 2^15. BF16 has the range as it is.
+template <typename M>
+constexpr float kProbUp = std::is_same<M, __half>::value ? 7.0f : 0.0f;
+
 // Division of 0 <= u < 2^27 (a 16-key block of a 31-bit length) by a page's blocks, as a product: m = 2^32 / d
 // rounded up is off by less than one in d · m, so u · m / 2^32 is exact while u · d < 2^32 (d <= 32, pages of up to 512
 // tokens) and larger pages divide.

@@ -574,7 +574,7 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
             }
           };
           float2 ls[2];  // the step's row sum, in four chains
-          // P of a chunk: 2^(x · sl2 − m), its sums in FP32 before the rounding to 16 bits
+          // P of a chunk: 2^(x · sl2 − base), its sums in FP32 before the rounding to 16 bits
           auto probabilities = [&](const float (&x)[32], float base, uint32_t (&pk)[16]) {
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
@@ -587,8 +587,10 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
           auto row_sum = [&] { return (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y); };
           // A step that every row of the warp sees whole, once there is a maximum to take the exponentials against: the
           // scores stay in registers. Only where a row's sum then shows that a score had passed the running maximum by
-          // much, the step's own is taken and the exponentials once more. P below 2^14 fits FP16, and its sums FP32.
+          // much, the step's own is taken and the exponentials once more. P is no larger than its row's sum: what
+          // kMost lets through fits FP16.
           if (C::HOLD && j >= open0 && j < open1 && !__any_sync(0xffffffffu, m == -INFINITY)) {
+            constexpr float kMost = std::is_same<M, __half>::value ? 65504.0f : 16384.0f;
             float s[NC][32];
 #pragma unroll
             for (int c = 0; c < NC; ++c) load(c, s[c]);
@@ -598,10 +600,10 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
 #pragma unroll
               for (int c = 0; c < NC; ++c) {
                 uint32_t pk[16];
-                probabilities(s[c], m, pk);
+                probabilities(s[c], m - kProbUp<M>, pk);
                 tmem_st_32x32b_x16(s_col + 16 * c, pk);
               }
-              if (again || !__any_sync(0xffffffffu, !(row_sum() <= 16384.0f))) break;
+              if (again || !__any_sync(0xffffffffu, !(row_sum() <= kMost))) break;
               again = true;
               float mx = s[0][0];
 #pragma unroll
@@ -643,7 +645,7 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
             }
             const float top = fmax3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * sl2;
             if (__any_sync(0xffffffffu, top > m + kTcLazy)) raise(top);
-            const float base = m == -INFINITY ? 0.0f : m;
+            const float base = (m == -INFINITY ? 0.0f : m) - kProbUp<M>;
             ls[0] = ls[1] = make_float2(0.0f, 0.0f);
 #pragma unroll 1
             for (int c = 0; c < NC; ++c) {

@@ -98,6 +98,43 @@ def test_visible_nans_reach_the_output(torch, kvcache, form, dim, bits, dtype):
         agree(got, w.expect(q, window, sinks), bar(w, dtype))
 
 
+@pytest.mark.parametrize("bits,dtype", [(16, "fp16"), (16, "bf16"), (4, "fp16"), (4, "bf16")])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 300, 37000])
+def test_many_small_probabilities_keep_their_weight(torch, kvcache, new, dim, bits, dtype):
+    # one key 18 above 131,000 others: each of them has a probability below FP16's smallest, 2^-25.97, and all together
+    # 1/500 of the output. One row's and 300 rows' keys are split over CTAs, most of which never meet the large one; those of
+    # 37,000 rows are not.
+    n, dt = 131072, dtype_of(torch, dtype)
+    pages = n // 1024
+    key, value = torch.zeros((n, 1, dim)), torch.ones((n, 1, dim))
+    key[0, 0, 0], value[0] = 2.25, 0.0
+    pools, scales, first = [], [], None
+    for x in (key, value):
+        x = x.to(dt)
+        if bits == 16:
+            pools.append(x.view(pages, 1024, 1, dim).transpose(1, 2).contiguous().cuda())
+            scales.append(None)
+            first = float(x[0, 0, 0]) if first is None else first
+        else:
+            c, s = quantise(torch, x)
+            first = float(values(torch, c[:1], s[:1])[0, 0, 0]) if first is None else first
+            pools.append(c.view(pages, 1024, 1, -1).transpose(1, 2).contiguous().cuda())
+            scales.append(s.view(pages, 1024, 1, -1, 2).transpose(1, 2).contiguous().cuda())
+    cache = kvcache.PagedCache.over(*pools, *scales)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    step = kvcache.Step(i32([n]), torch.arange(pages, dtype=torch.int32).view(1, -1).cuda(), n, i32([0, new]), new)
+    q = torch.zeros((new, 1, dim), dtype=dt)
+    q[..., 0] = 8.0
+    got = cache.attention(step, q.cuda(), scale=1.0).cpu().double()
+    sync()
+    others = torch.arange(n - new, n, dtype=torch.float64)
+    exp = (others / (others + math.exp(8.0 * first)))[:, None, None].expand_as(got)
+    err = float((got - exp).abs().max())
+    print(f"max error {err:.2e}, output {float(exp.max()):.2e}")
+    assert err <= 2 * ROUNDING[dtype] + 1e-4  # the bar, with max |v| = 1
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("form", FORMS)
