@@ -569,7 +569,8 @@ jc_status jc_kv_append_device(int device, jc_precision precision, const jc_kv_ca
  * j <= t with j > t - window or j < sinks (window 0: every j <= t);
  *   out [tokens, heads, D] = sum_j softmax_j(scale * q.k_j) v_j, zeros for a token that sees no key.
  * Query head h reads kv head h / (heads / kv_heads). Statistics and sums are held in FP32. Values in slots that a
- * token does not see never reach its output, whatever they are. `workspace` (16-byte aligned device memory, NULL
+ * token does not see never reach its output, whatever they are. `out` may be `q` itself; otherwise the two share no
+ * element. `workspace` (16-byte aligned device memory, NULL
  * when jc_kv_attention_workspace says 0) holds partial results during the call; its contents do not matter.
  */
 jc_status jc_kv_attention_device(int device, jc_precision precision, const jc_kv_cache* cache, const jc_kv_step* step,

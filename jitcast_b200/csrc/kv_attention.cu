@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 2 : BITS == 4 ? 4 : 3) 
       if (!on) {
         w[c][0] = w[c][1] = w[c][2] = w[c][3] = 0u;
       } else if (sh.vec_q) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + d));
+        const uint4 u = kv_load16(p + d);
         w[c][0] = u.x, w[c][1] = u.y, w[c][2] = u.z, w[c][3] = u.w;
       } else {
         const uint16_t* h = reinterpret_cast<const uint16_t*>(p + d);
@@ -484,8 +484,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 2 : BITS == 4 ? 4 : 3) 
   if (tid == 0) s_nan = 0u;
   __syncthreads();
   const bool whole = tl.kb.n <= sh.chunk;  // no other CTA has keys of this tile
-  for (int w = tid; w < tl.rows * (D / 4); w += 32 * kWarps) {
-    const int r = w / (D / 4), d = 4 * (w % (D / 4));
+  for (int w1 = 32 * warp; w1 < tl.rows * (D / 4); w1 += 32 * kWarps) {
+    const int w = w1 + lane;
+    const bool on = w < tl.rows * (D / 4);
+    const int r = on ? w / (D / 4) : 0, d = 4 * (w % (D / 4));
     float mm = s_m[0][r];
 #pragma unroll
     for (int k = 1; k < kWarps; ++k) mm = fmaxf(mm, s_m[k][r]);
@@ -505,9 +507,14 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 2 : BITS == 4 ? 4 : 3) 
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
       const bool none = sum == 0.0f && sq.length - sq.n + rr / group >= 0;  // a token of an index sees its own key at least
-      if (none || acc.x != acc.x || acc.y != acc.y || acc.z != acc.z || acc.w != acc.w) atomicOr(&s_nan, 1u << r);
-      store4(static_cast<T*>(a.out.p) + row * a.out.ld + head * a.out.hs + d, acc, sh.vec_o);
-    } else {
+      // A row to be worked out again is not stored, its q may lie where its output goes; a row's lanes are neighbours
+      const bool nan = none || acc.x != acc.x || acc.y != acc.y || acc.z != acc.z || acc.w != acc.w;
+      const uint32_t bad = __ballot_sync(0xffffffffu, on && nan) & (D == 128 ? ~0u : 0xFFFFu << (lane & 16));
+      if (on && bad == 0u)
+        store4(static_cast<T*>(a.out.p) + row * a.out.ld + head * a.out.hs + d, acc, sh.vec_o);
+      else if (on && d == 0)
+        atomicOr(&s_nan, 1u << r);
+    } else if (on) {
       *reinterpret_cast<float4*>(part_o(a, split, row * a.heads + head, D) + d) = acc;
       if (d == 0) *part_ml(a, sh.splits, split, row * a.heads + head, D) = make_float2(mm, sum);
     }
@@ -583,12 +590,13 @@ __global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
     bad = (sum == 0.0f && sq.length - sq.n + i >= 0) || acc.x != acc.x || acc.y != acc.y || acc.z != acc.z || acc.w != acc.w;
-    store4(static_cast<T*>(a.out.p) + (static_cast<long long>(sq.row0) + i) * a.out.ld + head * a.out.hs + 4 * d, acc, sh.vec_o);
   }
-  if (__syncthreads_or(bad) && warp == 0) {
-    const long long g = static_cast<long long>(sq.row0) + i;
-    kv_attend_row<T, BITS, D>(a, blockIdx.y, sq.length - sq.n + i, head, static_cast<const T*>(a.q.p) + g * a.q.ld + head * a.q.hs,
-                              static_cast<T*>(a.out.p) + g * a.out.ld + head * a.out.hs);
+  const long long g = static_cast<long long>(sq.row0) + i;
+  T* out = static_cast<T*>(a.out.p) + g * a.out.ld + head * a.out.hs;
+  if (!__syncthreads_or(bad)) {
+    if (tid < LANES) store4(out + 4 * d, acc, sh.vec_o);
+  } else if (warp == 0) {  // q is still there where the output goes to its place
+    kv_attend_row<T, BITS, D>(a, blockIdx.y, sq.length - sq.n + i, head, static_cast<const T*>(a.q.p) + g * a.q.ld + head * a.q.hs, out);
   }
 }
 

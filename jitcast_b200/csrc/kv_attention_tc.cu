@@ -324,7 +324,7 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
 #pragma unroll
       for (int c = 0; c < CH; ++c, at.next()) {
         const bool on = w0 + c * RPI + lane / CH < r0 + rows;  // a row past the last reads the first one, and is zeroed
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(base + (on ? at.tok * a.q.ld + at.rem * a.q.hs : 0)));
+        const uint4 u = kv_load16(base + (on ? at.tok * a.q.ld + at.rem * a.q.hs : 0));
         qv[c] = make_uint4(on ? u.x : 0u, on ? u.y : 0u, on ? u.z : 0u, on ? u.w : 0u);
       }
     } else {
@@ -732,6 +732,8 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
               *reinterpret_cast<uint4*>(qs + (c >> 1) * C::Q_ATOM + sw128(wrow + lane, 8 * (4 * (c & 1) + u))) =
                   make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
           }
+          // rows to be worked out again are not stored: their q may lie where their output goes
+          uint32_t redo = __ballot_sync(0xffffffffu, mine && nan);
           __syncwarp();
           {
             RowWalk at(w0 + lane / CH, RPI, group);
@@ -741,7 +743,7 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
               const int row = c * RPI + lane / CH;
               const uint4 v = *reinterpret_cast<const uint4*>(qs + (ch >> 3) * C::Q_ATOM + sw128(wrow + row, 8 * (ch & 7)));
               T* op = base + at.tok * a.out.ld + at.rem * a.out.hs;
-              if (w0 + row > w1) continue;
+              if (w0 + row > w1 || ((redo >> row) & 1u)) continue;
               if (tc.vec_o) {
                 *reinterpret_cast<uint4*>(op) = v;
               } else {
@@ -751,8 +753,6 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
               }
             }
           }
-          uint32_t redo = __ballot_sync(0xffffffffu, mine && nan);
-          __syncwarp();
           while (redo) {
             const int w = __ffs(redo) - 1;
             redo &= redo - 1;

@@ -83,6 +83,14 @@ __device__ __forceinline__ uint32_t kv_pack(float a, float b) {
   }
 }
 
+// 16 bytes of rows that the same kernel may write (a call in place): not the read-only path of __ldg. A thread's loads may
+// still move past other rows' stores, which are to other addresses.
+__device__ __forceinline__ uint4 kv_load16(const void* p) {
+  uint4 v;
+  asm("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // The smaller (larger) of two values, NaN if either is one.
 __device__ __forceinline__ float min_nan(float a, float b) {
   float r;

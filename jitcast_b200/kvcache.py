@@ -259,7 +259,8 @@ class PagedCache:
     def attention(self, step: Step, q, window: int = 0, sinks: int = 0, scale: float | None = None, out=None):
         """Attention of the step's new tokens ``q`` [tokens, heads, head_dim] over the cache, which holds their keys
         already: each sees the keys up to its own, within ``window`` of it (0: all) or among the sequence's first
-        ``sinks``. ``scale`` defaults to head_dim ** -0.5. Returns ``out`` (a new tensor by default)."""
+        ``sinks``. ``scale`` defaults to head_dim ** -0.5. Returns ``out`` (q itself, or a tensor beside it; a new one by
+        default)."""
         import torch
 
         self._check_step(step)

@@ -153,3 +153,20 @@ def test_rows_of_infinitely_small_scores(torch, kvcache, form, dim, dtype):
     exp = w.expect(q, 0, 0)
     assert exp[w.bounds[1]:].isnan().all() and not exp[:w.bounds[1]].isnan().any()
     agree(got, exp, bar(w, dtype))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kv,lengths,news", [(2, [90, 41], [3, 3]), (2, [9000, 41], [3, 3]), (8, [300, 70], [150, 3]),
+                                             (8, [4500, 200], [70, 45])])
+def test_out_may_be_q(torch, kvcache, kv, lengths, news, dim, bits):
+    # in place, with a value that only the last token sees undefined, so that the rows before it are worked out again
+    w = World(torch, kvcache, bits, "bf16", dim, kv, 64, lengths, news)
+    spoil(w, 1, 0, lengths[0] - 1)
+    spoil(w, 1, 1, lengths[1] - 1)
+    q = queries(torch, w, 2 * kv)
+    dev = q.cuda()
+    got = w.cache.attention(w.step(), dev, out=dev)
+    sync()
+    assert got is dev
+    agree(got, w.expect(q, 0, 0), bar(w, "bf16"))
