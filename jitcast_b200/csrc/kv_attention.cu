@@ -521,14 +521,12 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 2 ? 2 : BITS == 4 ? 4 : 3) 
   }
   if (!whole) return;
   __syncthreads();
-  for (int r = warp; r < tl.rows; r += kWarps)
-    if ((s_nan >> r) & 1u) {
-      const int rr = r0 + r, i = rr / group, head = kvh * group + rr % group;
-      const long long row = sq.row0 + i;
-      kv_attend_row<T, BITS, D>(a, seq, sq.length - sq.n + i, head,
-                                static_cast<const T*>(a.q.p) + row * a.q.ld + head * a.q.hs,
-                                static_cast<T*>(a.out.p) + row * a.out.ld + head * a.out.hs);
-    }
+  for (uint32_t left = s_nan; left; left &= left - 1) {  // the same for every thread
+    const int rr = r0 + __ffs(left) - 1, i = rr / group, head = kvh * group + rr % group;
+    const long long row = sq.row0 + i;
+    kv_attend_row_cta<T, BITS, D>(a, seq, sq.length - sq.n + i, head, static_cast<const T*>(a.q.p) + row * a.q.ld + head * a.q.hs,
+                                  static_cast<T*>(a.out.p) + row * a.out.ld + head * a.out.hs, &s_o[0][0][0], &s_m[0][0]);
+  }
 }
 
 // Joins the splits of an output row: a block a row, D / 4 threads a split at a time, the splits' weights first and
@@ -595,8 +593,9 @@ __global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__
   T* out = static_cast<T*>(a.out.p) + g * a.out.ld + head * a.out.hs;
   if (!__syncthreads_or(bad)) {
     if (tid < LANES) store4(out + 4 * d, acc, sh.vec_o);
-  } else if (warp == 0) {  // q is still there where the output goes to its place
-    kv_attend_row<T, BITS, D>(a, blockIdx.y, sq.length - sq.n + i, head, static_cast<const T*>(a.q.p) + g * a.q.ld + head * a.q.hs, out);
+  } else {  // q is still there where the output goes to its place
+    kv_attend_row_cta<T, BITS, D>(a, blockIdx.y, sq.length - sq.n + i, head,
+                                  static_cast<const T*>(a.q.p) + g * a.q.ld + head * a.q.hs, out, &s_acc[0][0].x, s_red);
   }
 }
 

@@ -108,16 +108,4 @@ __device__ __forceinline__ __half kv_code_value(uint32_t c, __half2 sm) {
   return __hfma(__ushort2half_rn(static_cast<unsigned short>(c)), __low2half(sm), __high2half(sm));
 }
 
-// Dim d of pool row `row` as FP32.
-template <typename T, int BITS>
-__device__ __forceinline__ float kv_value(const void* pool, const void* scale, long long row, int dim, int d) {
-  if constexpr (BITS == 16) {
-    return kv_float(static_cast<const T*>(pool)[row * dim + d]);
-  } else {
-    const uint8_t b = static_cast<const uint8_t*>(pool)[row * (dim / 2) + d / 2];
-    const __half2 sm = static_cast<const __half2*>(scale)[row * (dim / kKvGroup) + d / kKvGroup];
-    return __half2float(kv_code_value((d & 1) ? b >> 4 : b & 15, sm));
-  }
-}
-
 }  // namespace jc
