@@ -21,6 +21,7 @@
 #include <atomic>
 #include <cmath>
 
+#include "copies.h"
 #include "gemm.h"
 #include "kv_attention.cuh"
 
@@ -81,6 +82,13 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, const v
   while (!mbar_try_wait_long(bar, parity))
     if (*abort_flag || globaltimer() - t0 > kWaitLimitNs) return false;
   return true;
+}
+
+// Waits for a phase of what is in flight at the end, some 100 ms at most.
+__device__ __forceinline__ void last_wait(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < 100; ++i)
+    if (mbar_try_wait_long(bar, parity)) return;
 }
 
 __device__ __forceinline__ bool elect_one() {
@@ -252,7 +260,7 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
   uint64_t* o_full = p_full + 2;              // [2] MMA → softmax: every product of the tile done
   uint64_t* q_full = o_full + 2;              // [2] softmax → MMA: Q written (4 warps)
   uint64_t* v_raw = q_full + 2;               // [1] TMA → producer: a V tile with hidden rows to clear
-  uint64_t* drain = v_raw + 1;                // [1] MMA: products issued before it gave up
+  uint64_t* drain = v_raw + 1;                // [1] MMA: every product that it issued has completed
   uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile uint32_t* abort_flag = slot + 1;
 
@@ -374,6 +382,8 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
       const uint32_t off = atom * C::ATOM + blk * (size * 128);
       bool ok = true;
       uint32_t raw_phase = 0;
+      int k_sent = 0, v_sent = 0;  // steps whose copies complete on k_full, v_full
+      bool raw_sent = false;       // a V tile is on its way to v_raw
       int row = row_first;
       for (int j = 0; j < steps && ok; ++j) {
         const int st = j % C::STAGES;
@@ -385,6 +395,7 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
         if (lane == 0) mbar_arrive_expect_tx(k_full + st, C::TILE);
         __syncwarp();
         if (mine) tma_load_2d(smem + C::K_OFF + st * C::TILE + off, &tmK, k_full + st, 64 * atom, row);
+        k_sent = j + 1;
         ok = bar_wait(v_free + st, ph ^ 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -398,10 +409,11 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
         __syncwarp();
         if (mine) tma_load_2d(vt, &tmV, bar, 64 * atom, row);
         if (clear) {
-          ok = bar_wait(v_raw, raw_phase, abort_flag);
-          raw_phase ^= 1;
-          ok = __all_sync(0xffffffffu, ok);
+          raw_sent = true;
+          ok = __all_sync(0xffffffffu, bar_wait(v_raw, raw_phase, abort_flag));
           if (!ok) break;
+          raw_phase ^= 1;
+          raw_sent = false;
           for (uint32_t left = __ballot_sync(0xffffffffu, part); left; left &= left - 1) {
             const int from = __ffs(left) - 1;  // the whole warp clears that lane's block
             const int k0 = __shfl_sync(0xffffffffu, key0, from);
@@ -415,20 +427,20 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
           __syncwarp();
           if (lane == 0) mbar_arrive(v_full + st);
         }
+        v_sent = j + 1;
         row = next;
       }
-      if (!ok) {
-        if (lane == 0) {
+      if (lane == 0) {
+        if (!ok) {
           *abort_flag = 1;
           atomicOr(a.err, kErrAttnWait);
         }
-        // the copies in flight land before the CTA's shared memory can go
-        __syncwarp();
-        for (int i = 0; i < C::STAGES; ++i) {
-          mbar_wait(k_full + i, 0, 1000000);
-          mbar_wait(v_full + i, 0, 1000000);
-        }
+        // No copy is in flight when the CTA's shared memory can go, whichever role gave up
+        for_last_copies(k_sent, C::STAGES, [&](int i, uint32_t parity) { last_wait(k_full + i, parity); });
+        for_last_copies(v_sent, C::STAGES, [&](int i, uint32_t parity) { last_wait(v_full + i, parity); });
+        if (raw_sent) last_wait(v_raw, raw_phase);
       }
+      __syncwarp();
     } else if (warp == 9) {
       // ---- MMA issuer ----
       // The whole warp runs it, one elected lane issues: what the instructions take stays in uniform registers (with one
@@ -491,11 +503,13 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
             if (jn < steps) commit(k_free + jn % C::STAGES);
           }
         }
-        if (!ok && leader) {
-          *abort_flag = 1;
-          atomicOr(a.err, kErrAttnWait);
-          umma_commit(drain);  // every product issued has completed once this flips
-          mbar_wait(drain, 0, 1000000);
+        if (leader) {
+          if (!ok) {
+            *abort_flag = 1;
+            atomicOr(a.err, kErrAttnWait);
+          }
+          umma_commit(drain);  // every product issued has completed once this flips, whichever role gave up
+          last_wait(drain, 0);
         }
       }
       __syncwarp();
