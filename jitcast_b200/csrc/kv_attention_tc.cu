@@ -619,6 +619,7 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
               }
               if (again || !__any_sync(0xffffffffu, !(row_sum() <= kMost))) break;
               again = true;
+              tmem_st_wait();  // the same columns are written once more
               float mx = s[0][0];
 #pragma unroll
               for (int c = 0; c < NC; ++c)
