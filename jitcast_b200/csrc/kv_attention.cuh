@@ -107,12 +107,13 @@ __device__ __forceinline__ float kv_warp_max(float x) {
 // score is -inf (NaN, as 0 / 0 is).
 // Eight lanes take a key's row, so four whole rows a load; in step e the lanes 8 g .. 8 g + 7 have key 8 g + e, and keep its
 // score in lane 8 g + e. An undefined score makes the whole row undefined and ends the walk. (A prompt of 4,096 with every
-// row worked out again, 4 heads of 64: 4.1 ms, over 4 bits 5.0, where the call takes 0.08: the latencies of a group's chain, 32 rows
+// row worked out again, 4 heads of 64: 4.8 ms, over 4 bits 5.2, where the call takes 0.08: the latencies of a group's chain, 32 rows
 // a warp. Key after key it took 58 and 60, with a lane a key's row 6.6.)
 template <typename T, int BITS, int D>
 __device__ __forceinline__ void kv_attend_keys(const KvAttnArgs& a, int s, int t, int head, const T* q, int part, int parts,
                                                float& m, float& l, float (&o)[D / 64][8], bool& seen) {
   constexpr int N = D / 64;
+  constexpr int FLY = BITS == 16 && N == 2 ? 4 : 8;  // rows that a lane has in flight: 32 registers
   const int lane = threadIdx.x & 31, c = lane & 7, g8 = lane & 24;
   const int kvh = head / (a.heads / a.c.kv_heads);
   const int* table = a.st.table + s * a.st.ld_table;
@@ -147,27 +148,30 @@ __device__ __forceinline__ void kv_attend_keys(const KvAttnArgs& a, int s, int t
     seen = true;
     const int other = __shfl_sync(0xffffffffu, row, __ffs(there) - 1), from = row >= 0 ? row : other;
     int rows[8];
-    KvEight<T, BITS, D> raw[8][N];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      rows[e] = __shfl_sync(0xffffffffu, from, g8 + e);
-#pragma unroll
-      for (int i = 0; i < N; ++i) raw[e][i].load(a.c.k, a.c.k_scale, rows[e], 64 * i + 8 * c);
-    }
+    KvEight<T, BITS, D> raw[FLY][N];
     float d = 0.0f, v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float sum = 0.0f;
+    for (int e0 = 0; e0 < 8; e0 += FLY) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        raw[e][i].values(true, v);
+      for (int e = 0; e < FLY; ++e) {
+        rows[e0 + e] = __shfl_sync(0xffffffffu, from, g8 + e0 + e);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sum = fmaf(x[i][k], v[k], sum);
-        raw[e][i].load(a.c.v, a.c.v_scale, rows[e], 64 * i + 8 * c);  // in flight under the softmax
+        for (int i = 0; i < N; ++i) raw[e][i].load(a.c.k, a.c.k_scale, rows[e0 + e], 64 * i + 8 * c);
       }
 #pragma unroll
-      for (int w = 1; w < 8; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-      if (c == e) d = sum;
+      for (int e = 0; e < FLY; ++e) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          raw[e][i].values(true, v);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sum = fmaf(x[i][k], v[k], sum);
+          if (e0 + FLY == 8) raw[e][i].load(a.c.v, a.c.v_scale, rows[e], 64 * i + 8 * c);  // in flight under the softmax
+        }
+#pragma unroll
+        for (int w = 1; w < 8; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        if (c == e0 + e) d = sum;
+      }
     }
     const float mn = fmaxf(m, kv_warp_max(row >= 0 ? d : -INFINITY));
     const float up = mn == -INFINITY ? 1.0f : __expf(m - mn);  // -inf - -inf would be NaN
@@ -179,15 +183,18 @@ __device__ __forceinline__ void kv_attend_keys(const KvAttnArgs& a, int s, int t
       return;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float pe = __shfl_sync(0xffffffffu, p, g8 + e);
+    for (int e0 = 0; e0 < 8; e0 += FLY)
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        raw[e][i].values((there >> (g8 + e)) & 1u, v);
+      for (int e = 0; e < FLY; ++e) {
+        const float pe = __shfl_sync(0xffffffffu, p, g8 + e0 + e);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[i][k] = e == 0 ? fmaf(o[i][k], up, pe * v[k]) : fmaf(pe, v[k], o[i][k]);
+        for (int i = 0; i < N; ++i) {
+          raw[e][i].values((there >> (g8 + e0 + e)) & 1u, v);
+          if (e0 + FLY < 8) raw[e][i].load(a.c.v, a.c.v_scale, rows[FLY + e], 64 * i + 8 * c);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[i][k] = e0 + e == 0 ? fmaf(o[i][k], up, pe * v[k]) : fmaf(pe, v[k], o[i][k]);
+        }
       }
-    }
   }
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
@@ -202,7 +209,8 @@ __device__ __forceinline__ void kv_attend_keys(const KvAttnArgs& a, int s, int t
 // What a row's sum divides by.
 __device__ __forceinline__ float kv_inverse(float l, bool seen) { return l != 0.0f ? 1.0f / l : seen ? NAN : 0.0f; }
 
-// A row by one warp.
+// A row by one warp. (The tiles call it in one place, at their end: what it needs in registers cost them 2 to 6 % where it
+// was called in their middle.)
 template <typename T, int BITS, int D>
 __device__ __noinline__ void kv_attend_row(const KvAttnArgs& a, int s, int t, int head, const T* q, T* out) {
   const int lane = threadIdx.x & 31;

@@ -366,6 +366,7 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
   const bool good = __syncthreads_or(bad) == 0;
   tc_fence_after();
   const uint32_t tmem = *slot;
+  uint32_t redo = 0u;  // rows of the warp to be worked out again, key by key
 
   if (good && warp >= 8) {
     if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
@@ -748,7 +749,7 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
                   make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
           }
           // rows to be worked out again are not stored: their q may lie where their output goes
-          uint32_t redo = __ballot_sync(0xffffffffu, mine && nan);
+          redo = __ballot_sync(0xffffffffu, mine && nan);
           __syncwarp();
           {
             RowWalk at(w0 + lane / CH, RPI, group);
@@ -768,34 +769,28 @@ __global__ void __launch_bounds__((TcCfg<BITS, D, LONG>::THREADS), (TcCfg<BITS, 
               }
             }
           }
-          while (redo) {
-            const int w = __ffs(redo) - 1;
-            redo &= redo - 1;
-            const int xr = w0 + w, xt = xr / group, xh = kvh * group + xr % group;
-            const long long xg = static_cast<long long>(sq.row0) + xt;
-            kv_attend_row<T, BITS, D>(a, seq, base_t + xt, xh, static_cast<const T*>(a.q.p) + xg * a.q.ld + xh * a.q.hs,
-                                    static_cast<T*>(a.out.p) + xg * a.out.ld + xh * a.out.hs);
-          }
         }
       }
     }
-  } else {
-    for (int r = warp; r < rows; r += C::THREADS / 32) {
-      const int xr = r0 + r, xt = xr / group, xh = kvh * group + xr % group;
-      const long long xg = static_cast<long long>(sq.row0) + xt;
-      if (!whole) {  // the join recomputes a row whose sum is not a number
-        if (lane == 0) *part_ml(a, tc.splits, split, xg * a.heads + xh, D) = make_float2(0.0f, NAN);
-        continue;
-      }
-      kv_attend_row<T, BITS, D>(a, seq, base_t + xt, xh, static_cast<const T*>(a.q.p) + xg * a.q.ld + xh * a.q.hs,
-                              static_cast<T*>(a.out.p) + xg * a.out.ld + xh * a.out.hs);
-    }
+  } else if (warp < 8) {
+    const int r = w0 + lane;
+    if (whole)
+      redo = __ballot_sync(0xffffffffu, r < r0 + rows);
+    else if (r < r0 + rows)  // the join works a row out again whose sum is not a number
+      *part_ml(a, tc.splits, split, (static_cast<long long>(sq.row0) + r / group) * a.heads + kvh * group + r % group, D) =
+          make_float2(0.0f, NAN);
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM);
+  }
+  for (; redo; redo &= redo - 1) {
+    const int r = w0 + __ffs(redo) - 1, tok = r / group, head = kvh * group + r % group;
+    const long long row = static_cast<long long>(sq.row0) + tok;
+    kv_attend_row<T, BITS, D>(a, seq, base_t + tok, head, static_cast<const T*>(a.q.p) + row * a.q.ld + head * a.q.hs,
+                              static_cast<T*>(a.out.p) + row * a.out.ld + head * a.out.hs);
   }
 }
 
