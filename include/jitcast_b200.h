@@ -194,8 +194,9 @@ jc_status jc_time_attention_device(int device, jc_precision precision, const voi
                                    void* stream);
 
 /* Waits for all work on `device`, then returns and clears the device's kernel error word:
- * JC_ERR_TIMEOUT if a kernel's bounded wait gave up since the last call, JC_ERR_INVALID_ARG if a key/value cache
- * call met device arrays outside its bounds. */
+ * JC_ERR_TIMEOUT if a kernel's bounded wait gave up since the last call. The key/value cache calls have a word of their
+ * own, which this call alone reads and clears (after the other, where that has an error: at the next call):
+ * JC_ERR_INVALID_ARG if one of them met device arrays outside its bounds. */
 jc_status jc_device_sync(int device);
 
 /* ===================================================================================== */

@@ -136,7 +136,7 @@ jc_status jc_kv_append_device(int device, jc_precision precision, const jc_kv_ca
   if (!rt) return fail(JC_ERR_NO_DEVICE, why);
   DeviceScope dev(device);
   if (!dev.ok) return fail(JC_ERR_CUDA, "cannot select the device");
-  a.err = rt->err;
+  a.err = rt->kv_err;
   const cudaError_t e = launch_kv_append(a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? JC_OK : fail_cuda(e, "cache append launch");
 } catch (...) {
@@ -178,7 +178,7 @@ jc_status jc_kv_attention_device(int device, jc_precision precision, const jc_kv
   if (!rt) return fail(JC_ERR_NO_DEVICE, why);
   DeviceScope dev(device);
   if (!dev.ok) return fail(JC_ERR_CUDA, "cannot select the device");
-  a.err = rt->err;
+  a.err = rt->kv_err;
   const cudaError_t e = launch_kv_attention(a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? JC_OK : fail_cuda(e, "cache attention launch");
 } catch (...) {
@@ -200,7 +200,7 @@ jc_status jc_kv_read_device(int device, jc_precision precision, const jc_kv_cach
   if (!rt) return fail(JC_ERR_NO_DEVICE, why);
   DeviceScope dev(device);
   if (!dev.ok) return fail(JC_ERR_CUDA, "cannot select the device");
-  a.err = rt->err;
+  a.err = rt->kv_err;
   const cudaError_t e = launch_kv_read(a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? JC_OK : fail_cuda(e, "cache read launch");
 } catch (...) {

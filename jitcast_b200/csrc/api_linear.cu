@@ -409,7 +409,8 @@ jc_status jc_device_sync(int device) {
   cudaSetDevice(device);
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return fail_cuda(e, "device synchronize");
-  return take_device_error(rt);
+  const jc_status st = take_device_error(rt);
+  return st == JC_OK ? take_kv_error(rt) : st;
 }
 
 }  // extern "C"

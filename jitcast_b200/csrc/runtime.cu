@@ -53,13 +53,14 @@ DeviceRt* device_rt(int device, std::string* why) {
     cudaGetDevice(&prev);
     cudaError_t e = cudaSetDevice(device);
     if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&rt->stream, cudaStreamNonBlocking);
-    if (e == cudaSuccess) e = cudaMalloc(&rt->err, sizeof(uint32_t));
-    if (e == cudaSuccess) e = cudaMemset(rt->err, 0, sizeof(uint32_t));
+    if (e == cudaSuccess) e = cudaMalloc(&rt->err, 2 * sizeof(uint32_t));
+    if (e == cudaSuccess) e = cudaMemset(rt->err, 0, 2 * sizeof(uint32_t));
     cudaSetDevice(prev);
     if (e != cudaSuccess) {
       if (why) *why = std::string("device init: ") + cudaGetErrorString(e);
       return nullptr;
     }
+    rt->kv_err = rt->err + 1;
     g_rts[device] = std::move(rt);
     if (device < 64) g_made[device].store(g_rts[device].get(), std::memory_order_release);
   }
@@ -89,13 +90,13 @@ void* scratch(DeviceRt* rt, int slot, size_t bytes) {
   return p;
 }
 
-jc_status take_device_error(DeviceRt* rt) {
+static jc_status take_word(DeviceRt* rt, uint32_t* word) {
   uint32_t host = 0;
-  cudaError_t e = cudaMemcpyAsync(&host, rt->err, sizeof(uint32_t), cudaMemcpyDeviceToHost, rt->stream);
+  cudaError_t e = cudaMemcpyAsync(&host, word, sizeof(uint32_t), cudaMemcpyDeviceToHost, rt->stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(rt->stream);
   if (e != cudaSuccess) return fail_cuda(e, "reading the device error word");
   if (host) {
-    cudaMemsetAsync(rt->err, 0, sizeof(uint32_t), rt->stream);
+    cudaMemsetAsync(word, 0, sizeof(uint32_t), rt->stream);
     cudaStreamSynchronize(rt->stream);
     if (host == kErrKvStep)
       return fail(JC_ERR_INVALID_ARG, "a cache step's starts, lengths, pages or positions lie outside its call's bounds");
@@ -107,5 +108,9 @@ jc_status take_device_error(DeviceRt* rt) {
   }
   return JC_OK;
 }
+
+jc_status take_device_error(DeviceRt* rt) { return take_word(rt, rt->err); }
+
+jc_status take_kv_error(DeviceRt* rt) { return take_word(rt, rt->kv_err); }
 
 }  // namespace jc

@@ -19,6 +19,8 @@ struct DeviceRt {
   std::mutex mu;
   cudaStream_t stream = nullptr;
   uint32_t* err = nullptr;  // device word; kernels atomicOr DeviceError bits into it
+  // The key/value cache calls' own: a caller's data can set it, so no other call may take it for its own error.
+  uint32_t* kv_err = nullptr;
   std::vector<void*> slot_ptr;
   std::vector<size_t> slot_bytes;
 };
@@ -42,6 +44,9 @@ jc_status fail_cuda(cudaError_t e, const char* what);
 
 // Reads and clears the device error word (synchronises rt->stream first).
 jc_status take_device_error(DeviceRt* rt);
+
+// The same for the cache calls' word.
+jc_status take_kv_error(DeviceRt* rt);
 
 inline long long round_up(long long x, long long m) { return (x + m - 1) / m * m; }
 

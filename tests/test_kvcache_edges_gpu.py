@@ -198,3 +198,19 @@ def test_an_undefined_value_does_not_stall_a_call(torch, kvcache, bits):
     print(f"{clean:.3f} ms, with every row worked out again {redone:.3f} ms")
     assert bool(out[:, :, 5].isnan().all())
     assert redone < 100 * clean
+
+
+def test_another_callers_product_does_not_take_a_cache_error(torch, kvcache, jc):
+    import numpy as np
+
+    w = World(torch, kvcache, 16, "fp16", 64, 2, 32, [64], [1])
+    bad = kvcache.Step(torch.tensor([65], dtype=torch.int32).cuda(), w.table.cuda(), 64)
+    q = torch.zeros((1, 2, 64), dtype=w.dt).cuda()
+    w.cache.attention(bad, q)
+    torch.cuda.synchronize()
+    x = np.ones((4, 64), np.float32)
+    y = jc.ops.linear(x, x, np.zeros(4, np.float32), precision="bf16")  # a right product
+    assert (y == 64).all()
+    with pytest.raises(_lib.JcArgumentError):  # and the cache's caller hears of its own error
+        sync()
+    sync()
