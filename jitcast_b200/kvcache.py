@@ -83,12 +83,17 @@ class Step:
     """The sequences of a call, shared by a model's layers: each one's cached ``length`` [n] (new tokens included)
     and its pages ``page_table`` [n, most pages], int32 on the GPU. ``start`` [n + 1] has the bounds of each
     sequence's packed new tokens; without it every sequence has one. ``max_length`` and ``max_new`` bound the
-    lengths and the new tokens. The tensors may be rewritten between calls (they are read on the GPU)."""
+    lengths and the new tokens, and may be set anew as series grow. The tensors stay those of the start; what they hold
+    may be rewritten between calls (they are read on the GPU)."""
+
+    length = property(lambda self: self._length)
+    page_table = property(lambda self: self._page_table)
+    start = property(lambda self: self._start)
 
     def __init__(self, length, page_table, max_length: int, start=None, max_new: int = 1):
-        self.length = _int32(length, "length", 1)
+        self._length = _int32(length, "length", 1)
         self.device = length.device
-        self.page_table = _int32(page_table, "page_table", 2, self.device)
+        self._page_table = _int32(page_table, "page_table", 2, self.device)
         n = length.shape[0]
         if page_table.shape[0] != n:
             raise ValueError(f"page_table has {page_table.shape[0]} rows for {n} sequences")
@@ -96,11 +101,31 @@ class Step:
             _int32(start, "start", 1, self.device)
             if start.shape[0] != n + 1:
                 raise ValueError(f"start has {start.shape[0]} bounds for {n} sequences")
-        elif max_new != 1:
+        self._start, self.sequences = start, n
+        self.max_length, self.max_new = max_length, max_new
+
+    @property
+    def max_length(self) -> int:
+        return self._max_length
+
+    @max_length.setter
+    def max_length(self, value: int) -> None:
+        if value < 0:
+            raise ValueError("max_length must be >= 0")
+        self._max_length = int(value)
+        self._by_tokens = {}
+
+    @property
+    def max_new(self) -> int:
+        return self._max_new
+
+    @max_new.setter
+    def max_new(self, value: int) -> None:
+        if self._start is None and value != 1:
             raise ValueError("a step without start has one new token per sequence")
-        if max_length < 0 or max_new < 0:
-            raise ValueError("max_length and max_new must be >= 0")
-        self.start, self.sequences, self.max_length, self.max_new = start, n, int(max_length), int(max_new)
+        if value < 0:
+            raise ValueError("max_new must be >= 0")
+        self._max_new = int(value)
         self._by_tokens = {}
 
     def _c(self, tokens: int):
@@ -120,7 +145,12 @@ class Step:
 class PagedCache:
     """One layer's keys and values in pages of ``page_size`` tokens. ``k`` and ``v`` are the pools
     [pages, kv_heads, page_size, head_dim] (``bits`` 16) or their codes [.., head_dim // 2] with
-    ``k_scale`` and ``v_scale`` [.., head_dim // 32, 2] (``bits`` 4)."""
+    ``k_scale`` and ``v_scale`` [.., head_dim // 32, 2] (``bits`` 4), the same tensors for as long as it lives."""
+
+    k = property(lambda self: self._pools[0])
+    v = property(lambda self: self._pools[1])
+    k_scale = property(lambda self: self._pools[2])
+    v_scale = property(lambda self: self._pools[3])
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=None, bits: int = 16,
                  device="cuda"):
@@ -168,7 +198,7 @@ class PagedCache:
         for t in (k, v, k_scale, v_scale):
             if t is not None and (not t.is_cuda or t.device != k.device or not t.is_contiguous()):
                 raise ValueError("pools and scales must be contiguous CUDA tensors on one device")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._pools = (k, v, k_scale, v_scale)
         self.pages, self.kv_heads, self.page_size, self.head_dim = *k.shape[:3], dim
         self.device = k.device
         self.dtype = k.dtype if self.bits == 16 else None

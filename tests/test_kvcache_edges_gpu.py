@@ -214,3 +214,27 @@ def test_another_callers_product_does_not_take_a_cache_error(torch, kvcache, jc)
     with pytest.raises(_lib.JcArgumentError):  # and the cache's caller hears of its own error
         sync()
     sync()
+
+
+def test_a_steps_bounds_may_grow_and_its_tensors_stay(torch, kvcache):
+    w = World(torch, kvcache, 16, "fp16", 64, 2, 32, [90], [1])
+    q = queries(torch, w, 2)
+    length = torch.tensor([40], dtype=torch.int32).cuda()
+    step = kvcache.Step(length, w.table.cuda(), 40)
+    w.cache.attention(step, q.cuda())
+    sync()
+    length.fill_(90)
+    step.max_length = 90
+    got = w.cache.attention(step, q.cuda())
+    sync()
+    assert float((got.cpu().double() - w.expect(q, 0, 0)).abs().max()) <= bar(w, "fp16")
+    for change in (lambda: setattr(step, "max_length", -1), lambda: setattr(step, "max_new", 2)):
+        with pytest.raises(ValueError):
+            change()
+    assert (step.max_length, step.max_new) == (90, 1)
+    # what a call reads stays what it was made of
+    for change in (lambda: setattr(step, "length", length.clone()), lambda: setattr(step, "page_table", w.table.cuda()),
+                   lambda: setattr(step, "start", length), lambda: setattr(w.cache, "k", w.cache.k.clone()),
+                   lambda: setattr(w.cache, "v_scale", None)):
+        with pytest.raises(AttributeError):
+            change()
