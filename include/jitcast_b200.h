@@ -541,8 +541,9 @@ typedef struct jc_kv_step {
 } jc_kv_step;
 
 /* Rows of heads on the device in the call's precision: element (row, head, dim) at row * ld + head * head_stride +
- * dim elements (a column block of a q|k|v product is such a tensor). Any strides whose heads do not overlap (and, of
- * rows that a call writes, whose rows do not); 16-byte aligned ones are faster. */
+ * dim elements (a column block of a q|k|v product is such a tensor). Any strides whose heads do not overlap; of rows that
+ * a call writes, all heads of a row lie before the next row, or all rows of a head before the next head. 16-byte aligned
+ * ones are faster. */
 typedef struct jc_kv_rows {
   void* data;
   long long ld;

@@ -76,12 +76,17 @@ jc_status check_rows(const jc_kv_rows* r, const char* name, int dim, int heads, 
   return JC_OK;
 }
 
-// Rows that a call writes: no two tokens may share an element.
-jc_status check_out(const jc_kv_rows* r, const char* name, int dim, int heads, KvRows* out) {
+// Rows that a call writes: no two tokens or heads may share an element. Either a token's heads lie within its pitch, or a
+// head's tokens do (heads before tokens).
+jc_status check_out(const jc_kv_rows* r, const char* name, int dim, int heads, int tokens, KvRows* out) {
   if (jc_status st = check_rows(r, name, dim, heads, out)) return st;
-  const long long span = heads > 1 ? static_cast<long long>(heads - 1) * r->head_stride + dim : dim;
-  if (r->ld < span) return fail(JC_ERR_INVALID_ARG, std::string(name) + " rows overlap");
-  return JC_OK;
+  if (tokens < 2) return JC_OK;
+  // n rows of `dim` elements, `inner` apart, fit into `pitch`
+  auto within = [dim](long long pitch, int n, long long inner) {
+    return pitch >= dim && (n < 2 || inner <= (pitch - dim) / (n - 1));
+  };
+  if (within(r->ld, heads, r->head_stride) || (r->ld >= dim && within(r->head_stride, tokens, r->ld))) return JC_OK;
+  return fail(JC_ERR_INVALID_ARG, std::string(name) + " rows overlap");
 }
 
 jc_status check_attention(jc_precision precision, const jc_kv_cache* cache, const jc_kv_step* step, int heads,
@@ -118,7 +123,7 @@ jc_status jc_kv_append_device(int device, jc_precision precision, const jc_kv_ca
     if (q) {
       if (heads < 1) return fail(JC_ERR_INVALID_ARG, "heads must be >= 1 with q");
       if (jc_status st = check_rows(q, "q", a.c.dim, heads, &a.q)) return st;
-      if (jc_status st = check_out(q_out, "q_out", a.c.dim, heads, &a.q_out)) return st;
+      if (jc_status st = check_out(q_out, "q_out", a.c.dim, heads, a.st.tokens, &a.q_out)) return st;
       a.heads = heads;
     }
   }
@@ -164,7 +169,7 @@ jc_status jc_kv_attention_device(int device, jc_precision precision, const jc_kv
   if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(JC_ERR_INVALID_ARG, "scale must be positive and finite");
   if (a.st.tokens > 0) {
     if (jc_status st = check_rows(q, "q", a.c.dim, heads, &a.q)) return st;
-    if (jc_status st = check_out(out, "out", a.c.dim, heads, &a.out)) return st;
+    if (jc_status st = check_out(out, "out", a.c.dim, heads, a.st.tokens, &a.out)) return st;
   }
   const long long need = kv_attention_workspace(a);
   if (need > 0 && (!workspace || workspace_bytes < need))
@@ -192,8 +197,8 @@ jc_status jc_kv_read_device(int device, jc_precision precision, const jc_kv_cach
   if (jc_status st = check_cache(precision, cache, &a.c)) return st;
   if (jc_status st = check_step(step, &a.st)) return st;
   if (a.st.tokens > 0) {
-    if (jc_status st = check_out(k, "k", a.c.dim, a.c.kv_heads, &a.k)) return st;
-    if (jc_status st = check_out(v, "v", a.c.dim, a.c.kv_heads, &a.v)) return st;
+    if (jc_status st = check_out(k, "k", a.c.dim, a.c.kv_heads, a.st.tokens, &a.k)) return st;
+    if (jc_status st = check_out(v, "v", a.c.dim, a.c.kv_heads, a.st.tokens, &a.v)) return st;
   }
   std::string why;
   DeviceRt* rt = device_rt(device, &why);

@@ -238,3 +238,22 @@ def test_a_steps_bounds_may_grow_and_its_tensors_stay(torch, kvcache):
                    lambda: setattr(w.cache, "v_scale", None)):
         with pytest.raises(AttributeError):
             change()
+
+
+@pytest.mark.parametrize("new", [1, 3, 150])
+def test_outputs_of_heads_before_tokens(torch, kvcache, new):
+    # [heads, tokens, dim] tensors seen as [tokens, heads, dim]: rows that do not overlap, in the other order
+    w = World(torch, kvcache, 16, "bf16", 64, 2, 64, [200], [new])
+    q = queries(torch, w, 6)
+    like = lambda x: x.cuda().transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    dev, out = like(q), like(torch.zeros_like(q))
+    got = w.cache.attention(w.step(), dev, out=out)
+    sync()
+    assert got is out
+    assert float((out.cpu().double() - w.expect(q, 0, 0)).abs().max()) <= bar(w, "bf16")
+    k = queries(torch, w, 2, 3)
+    out.zero_()
+    w.cache.append(w.step(), like(k), like(k), q=dev, q_out=out)
+    sync()
+    assert torch.equal(out.cpu(), q)
+    assert torch.equal(w.cache.read(w.step(), new)[0].cpu(), k)
