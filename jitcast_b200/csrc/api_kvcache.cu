@@ -62,7 +62,9 @@ jc_status check_step(const jc_kv_step* s, KvStep* out) {
     return fail(JC_ERR_INVALID_ARG, "a step without starts has one new token per sequence");
   if (s->sequences > 0 && (!s->length || (s->table_pages > 0 && !s->page_table)))
     return fail(JC_ERR_INVALID_ARG, "null length or page table");
-  *out = KvStep{s->sequences, s->tokens, s->max_new, s->max_length, s->start, s->length, s->page_table, s->table_pages,
+  // no sequence has more new tokens than there are rows: a looser bound shapes no launch and sizes no workspace
+  const int max_new = s->max_new < s->tokens ? s->max_new : s->tokens;
+  *out = KvStep{s->sequences, s->tokens, max_new, s->max_length, s->start, s->length, s->page_table, s->table_pages,
                 s->ld_table};
   return JC_OK;
 }
@@ -95,9 +97,8 @@ jc_status check_attention(jc_precision precision, const jc_kv_cache* cache, cons
   if (jc_status st = check_step(step, &a->st)) return st;
   if (heads < 1 || heads % a->c.kv_heads != 0) return fail(JC_ERR_INVALID_ARG, "heads must be a multiple of kv_heads");
   if (heads > 65535) return fail(JC_ERR_UNSUPPORTED_SHAPE, "at most 65535 heads");
-  const long long group = heads / a->c.kv_heads;
-  if (a->st.max_new * group > (1 << 30) || a->st.max_new * group / 256 * a->c.kv_heads > (1 << 30))
-    return fail(JC_ERR_UNSUPPORTED_SHAPE, "above 2^30 query rows");
+  if (static_cast<long long>(a->st.max_new) * heads > (1 << 30))
+    return fail(JC_ERR_UNSUPPORTED_SHAPE, "above 2^30 query rows of a sequence");
   if (window < 0 || sinks < 0) return fail(JC_ERR_INVALID_ARG, "window and sinks must be >= 0");
   a->heads = heads;
   a->window = window;
