@@ -31,7 +31,7 @@ template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const KvRows& r, long long token, int head, int d, float (&x)[8]) {
   const T* p = static_cast<const T*>(r.p) + token * r.ld + head * r.hs + d;
   if constexpr (VEC) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 u = kv_load16(p);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
