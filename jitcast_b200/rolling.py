@@ -22,20 +22,43 @@ class Pages:
     def __init__(self, series: int, pages: int, page_size: int, most_tokens: int, device="cuda"):
         import torch
 
-        self.page_size, self.free = page_size, list(range(pages - 1, -1, -1))
+        self.page_size, self.pages, self.free, self.peak = page_size, pages, list(range(pages - 1, -1, -1)), 0
         columns = -(-most_tokens // page_size)
-        self.host = torch.full((series, columns), -1, dtype=torch.int32).pin_memory()
         self.table = torch.full((series, columns), -1, dtype=torch.int32, device=device)
+        self.pinned = torch.full((series, columns), -1, dtype=torch.int32)
+        if self.table.is_cuda:
+            self.pinned = self.pinned.pin_memory()
+        self.host = self.pinned.numpy()  # -1 where no page is, or no longer
+        self.given = [0] * series  # columns handed out so far; those that were left stay without a page
+        self.left = [0] * series   # columns looked at for leaving
+
+    @staticmethod
+    def most(tokens: int, page_size: int, window: int = 0, sinks: int = 0, chunk: int = 1) -> int:
+        """The most pages that a series of ``tokens`` holds when it grows by up to ``chunk`` at a time."""
+        whole = -(-tokens // page_size)
+        if not window:
+            return whole
+        # the sinks' pages, and a band of window - 1 + chunk tokens that starts anywhere in a page
+        return min(whole, -(-sinks // page_size) + (window - 1 + chunk + page_size - 2) // page_size + 1)
+
+    @property
+    def used(self) -> int:
+        return self.pages - len(self.free)
 
     def grow(self, lengths) -> None:
         """Pages for series of these lengths (host integers), taken from the free ones."""
-        for s, length in enumerate(lengths):
-            for c in range(-(-length // self.page_size)):
-                if self.host[s, c] < 0:
-                    if not self.free:
-                        raise RuntimeError("the cache has no free page left")
-                    self.host[s, c] = self.free.pop()
-        self.table.copy_(self.host, non_blocking=True)
+        need = [-(-length // self.page_size) for length in lengths]
+        if sum(max(0, n - g) for n, g in zip(need, self.given)) > len(self.free):
+            raise RuntimeError("the cache has no free page left")
+        changed = False
+        for s, n in enumerate(need):
+            for c in range(self.given[s], n):
+                self.host[s, c] = self.free.pop()
+                changed = True
+            self.given[s] = max(self.given[s], n)
+        self.peak = max(self.peak, self.used)
+        if changed:
+            self.table.copy_(self.pinned, non_blocking=True)
 
     def leave(self, lengths, window: int, sinks: int) -> None:
         """Frees the pages that no later token of these series can see."""
@@ -43,10 +66,11 @@ class Pages:
             return
         first = -(-sinks // self.page_size)
         for s, length in enumerate(lengths):
-            for c in range(first, max(0, length + 1 - window) // self.page_size):
-                if self.host[s, c] >= 0:
-                    self.free.append(int(self.host[s, c]))
-                    self.host[s, c] = -1
+            last = min(max(0, length + 1 - window) // self.page_size, self.given[s])
+            for c in range(max(first, self.left[s]), last):
+                self.free.append(int(self.host[s, c]))
+                self.host[s, c] = -1
+            self.left[s] = max(self.left[s], last)
 
 
 class RollingTimeAttention:
@@ -101,7 +125,8 @@ def run(layers, pages: Pages, tokens, chunks):
 
 
 def demo(series=16, patches=300, prompt=130, heads=4, dim=64, depth=2, bits=16, window=0, sinks=0, page_size=64, seed=0):
-    """(outputs fed patch by patch after a prompt, outputs of everything at once, most pages in use)."""
+    """(outputs fed patch by patch after a prompt, outputs of everything at once, most pages in use). The pool of the first
+    holds what its window needs and no more."""
     import torch
 
     d, dev = heads * dim, "cuda"
@@ -110,16 +135,16 @@ def demo(series=16, patches=300, prompt=130, heads=4, dim=64, depth=2, bits=16, 
     weights = [(rand(3 * d, d) * d ** -0.5, rand(d, d) * d ** -0.5) for _ in range(depth)]
     tokens = rand(series, patches, d)
     rope = rope_table(patches, dim, dim // 4)
-    most = series * -(-patches // page_size)
 
-    def build():
+    def build(chunk):
+        most = series * max(Pages.most(patches, page_size, window, sinks), Pages.most(chunk, page_size))
         return [RollingTimeAttention(wq, wo, heads, most, page_size, bits, window, sinks, rope, dim // 4)
                 for wq, wo in weights], Pages(series, most, page_size, patches)
 
-    layers, pages = build()
+    layers, pages = build(prompt)
     rolled = run(layers, pages, tokens, [prompt] + [1] * (patches - prompt))
-    used = most - len(pages.free)
-    layers, pages = build()
+    used = pages.peak
+    layers, pages = build(patches)
     return rolled, run(layers, pages, tokens, [patches]), used
 
 
@@ -133,7 +158,7 @@ def main() -> None:
     ops.device_sync()
     err = float((rolled - whole).norm() / whole.norm())
     print(f"{args['series']} series of {args['patches']} patches, {args['prompt']} at once and then one by one: "
-          f"{err:.2e} from all at once (relative, 2-norm); {used} pages in use at the end")
+          f"{err:.2e} from all at once (relative, 2-norm); {used} pages in use at most")
 
 
 if __name__ == "__main__":

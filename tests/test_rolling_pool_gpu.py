@@ -1,0 +1,18 @@
+"""The rolling forecast on a pool that holds what its window needs, over several windows' worth of patches, against the same
+layers fed all at once on a pool for everything. The bars are those of test_rolling_gpu.py."""
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits,bar", [(16, 1e-2), (4, 2e-2)])
+def test_a_windows_pool_over_many_windows(jc, bits, bar):
+    pytest.importorskip("torch")
+    from jitcast_b200 import ops, rolling
+
+    rolled, whole, used = rolling.demo(series=3, patches=700, prompt=60, heads=2, dim=64, bits=bits, window=100, sinks=3,
+                                       page_size=32)
+    ops.device_sync()
+    assert used <= 3 * (1 + 5)  # of 22 pages a series
+    assert float((rolled - whole).norm() / whole.norm()) < bar
