@@ -17,18 +17,18 @@ from .kvcache import PagedCache, Step, rope_table
 
 
 class Pages:
-    """Page numbers of a pool shared by the layers (page p of every layer's cache belongs together)."""
+    """Page numbers of a pool shared by the layers (page p of every layer's cache belongs together). ``grow`` and ``leave``
+    work on the host and may run ahead of the GPU: a step enqueued after a ``grow`` reads the table of that ``grow``."""
 
     def __init__(self, series: int, pages: int, page_size: int, most_tokens: int, device="cuda"):
         import torch
 
         self.page_size, self.pages, self.free, self.peak = page_size, pages, list(range(pages - 1, -1, -1)), 0
         columns = -(-most_tokens // page_size)
+        # [series, columns]: -1 where no page is, or no longer
+        self.host = torch.full((series, columns), -1, dtype=torch.int32).numpy()
         self.table = torch.full((series, columns), -1, dtype=torch.int32, device=device)
-        self.pinned = torch.full((series, columns), -1, dtype=torch.int32)
-        if self.table.is_cuda:
-            self.pinned = self.pinned.pin_memory()
-        self.host = self.pinned.numpy()  # -1 where no page is, or no longer
+        self.pinned = self.table.is_cuda
         self.given = [0] * series  # columns handed out so far; those that were left stay without a page
         self.left = [0] * series   # columns looked at for leaving
 
@@ -47,6 +47,8 @@ class Pages:
 
     def grow(self, lengths) -> None:
         """Pages for series of these lengths (host integers), taken from the free ones."""
+        import torch
+
         need = [-(-length // self.page_size) for length in lengths]
         if sum(max(0, n - g) for n, g in zip(need, self.given)) > len(self.free):
             raise RuntimeError("the cache has no free page left")
@@ -58,10 +60,12 @@ class Pages:
             self.given[s] = max(self.given[s], n)
         self.peak = max(self.peak, self.used)
         if changed:
-            self.table.copy_(self.pinned, non_blocking=True)
+            # a buffer of its own for each copy, which may run after the host's table has changed again
+            now = torch.from_numpy(self.host).clone()
+            self.table.copy_(now.pin_memory() if self.pinned else now, non_blocking=True)
 
     def leave(self, lengths, window: int, sinks: int) -> None:
-        """Frees the pages that no later token of these series can see."""
+        """Frees the pages that no later token of these series can see, for tokens of steps enqueued after this call."""
         if not window:
             return
         first = -(-sinks // self.page_size)
@@ -119,7 +123,6 @@ def run(layers, pages: Pages, tokens, chunks):
         for layer in layers:
             x = layer(x, step)
         out.append(x.view(series, n, d))
-        torch.cuda.current_stream().synchronize()  # the host's table is rewritten below and by the next chunk
         pages.leave([done] * series, layers[0].window, layers[0].sinks)
     return torch.cat(out, 1)
 

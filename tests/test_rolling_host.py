@@ -58,3 +58,19 @@ def test_uneven_series_and_a_full_pool():
     assert pages.used == 4
     pages.grow([48, 20, 17])
     assert pages.used == 6 and int((pages.table[1] >= 0).sum()) == 2
+
+
+def test_what_a_step_reads_is_not_rewritten_under_it():
+    # a copy that runs late, as one enqueued behind other work does: the table that it brings is the one of its grow
+    class Late:
+        def copy_(self, src, non_blocking=False):
+            self.src = src
+
+    pages = Pages(1, 9, 16, 300, device="cpu")
+    pages.grow([90])
+    first = pages.table.clone()
+    pages.table = late = Late()
+    pages.grow([110])
+    pages.leave([110], 20, 0)  # most of the pages that the step just enqueued sees at its first tokens
+    assert int((late.src[0] >= 0).sum()) == 7
+    assert late.src[0, :6].tolist() == first[0, :6].tolist()

@@ -16,3 +16,20 @@ def test_a_windows_pool_over_many_windows(jc, bits, bar):
     ops.device_sync()
     assert used <= 3 * (1 + 5)  # of 22 pages a series
     assert float((rolled - whole).norm() / whole.norm()) < bar
+
+
+def test_pages_may_run_ahead_of_the_gpu(jc):
+    # tables and frees enqueued behind other work: each step reads the table of its own grow
+    torch = pytest.importorskip("torch")
+    from jitcast_b200 import rolling
+
+    pages = rolling.Pages(2, 40, 16, 4000)
+    got, want = [], []
+    torch.cuda._sleep(200_000_000)  # some 0.1 s of work before the first copy
+    for length in range(90, 1500, 10):
+        pages.grow([length, length])
+        got.append(pages.table.clone())
+        want.append(pages.host.copy())
+        pages.leave([length, length], 40, 16)
+    torch.cuda.synchronize()
+    assert all((g.cpu().numpy()[w >= 0] == w[w >= 0]).all() for g, w in zip(got, want))
