@@ -97,7 +97,8 @@ class RollingTimeAttention:
         n, d = x.shape
         qkv = torch.empty((n, 3 * d), dtype=torch.float32, device=x.device)
         ops.linear_device(x, self.w_qkv, None, qkv, 0, "fp16")
-        q, k, v = qkv.half().view(n, 3, self.heads, self.dim).unbind(1)
+        # the FP16 of the engines: saturated
+        q, k, v = qkv.clamp_(-65504.0, 65504.0).half().view(n, 3, self.heads, self.dim).unbind(1)
         q = self.cache.append(step, k, v, q=q, rope=self.rope, pairs=self.pairs)
         o = self.cache.attention(step, q, window=self.window, sinks=self.sinks)
         y = x.clone()

@@ -33,3 +33,21 @@ def test_pages_may_run_ahead_of_the_gpu(jc):
         pages.leave([length, length], 40, 16)
     torch.cuda.synchronize()
     assert all((g.cpu().numpy()[w >= 0] == w[w >= 0]).all() for g, w in zip(got, want))
+
+
+def test_projections_past_fp16_saturate(jc):
+    # keys of 1e5 are held as 65504, as the engines hold them: an infinity that rotates by a sine of 0 is undefined
+    torch = pytest.importorskip("torch")
+    from jitcast_b200 import kvcache, ops, rolling
+
+    w_qkv = torch.zeros((3 * 64, 64), device="cuda")
+    w_qkv[64, 0] = 1e5 / 8
+    w_qkv[128:, 0] = 1.0 / 8
+    layer = rolling.RollingTimeAttention(w_qkv, torch.eye(64, device="cuda"), 1, 1, rope=kvcache.rope_table(4, 64))
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    x = torch.zeros((1, 64), device="cuda")
+    x[0, 0] = 8.0
+    y = layer(x, kvcache.Step(i32([1]), i32([[0]]), 1))
+    ops.device_sync()
+    assert float(layer.cache.k[0, 0, 0, 0]) == 65504.0
+    assert torch.equal(y - x, torch.ones_like(x))
