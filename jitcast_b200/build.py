@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import concurrent.futures
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -22,7 +23,14 @@ INCLUDE = HERE.parent / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-Xptxas",
-         "-warn-spills"]
+         "-warn-spills", "-Xptxas", "-v"]
+
+# Registers a thread that kernels have to be launched with: their warpgroups share them out anew (setmaxnreg), and shares that
+# do not add up to the launch's would wait for ever. A compiler that gives another number fails here, not in the calls.
+REGISTERS = {
+    "kv_attention_tc.cu": [(r"kv_attention_tc_kernel\w*Li16ELi(?:64|128)ELi1E", 168),
+                           (r"kv_attention_tc_kernel\w*Li4ELi(?:64|128)ELi1E", 128)],
+}
 
 
 def nvcc() -> str:
@@ -43,6 +51,17 @@ def _stale(obj: Path, src: Path, deps: list[Path]) -> bool:
     return any(p.stat().st_mtime > t for p in [src, *deps])
 
 
+def check_registers(name: str, log: str) -> None:
+    """Holds the register counts of ptxas's report on source file `name` to REGISTERS."""
+    wanted = REGISTERS.get(name, [])
+    used = re.findall(r"Compiling entry function '(\w+)'.*?Used (\d+) registers", log, re.S)
+    for pattern, count in wanted:
+        found = [(f, int(n)) for f, n in used if re.search(pattern, f)]
+        wrong = [(f, n) for f, n in found if n != count]
+        if wrong or not found:
+            raise RuntimeError(f"{name}: {pattern} needs {count} registers a thread, the compiler gave {wrong or 'none'}")
+
+
 def _compile(src: Path, obj: Path, verbose: bool) -> None:
     cmd = [nvcc(), *ARCH, *FLAGS, "-I", str(INCLUDE), "-c", str(src), "-o", str(obj)]
     if verbose:
@@ -50,8 +69,10 @@ def _compile(src: Path, obj: Path, verbose: bool) -> None:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"nvcc failed on {src.name}:\n{r.stdout}\n{r.stderr}")
-    if "spill" in r.stderr and "0 bytes spill" not in r.stderr:
-        print(r.stderr, file=sys.stderr)
+    check_registers(src.name, r.stderr)
+    spilled = [line for line in r.stderr.splitlines() if "spilled" in line]
+    if spilled:
+        print("\n".join(spilled), file=sys.stderr)
 
 
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
