@@ -494,8 +494,8 @@ jc_status jc_chronos2_finish_device(int device, int rows, int output_patches, in
 /*
  * No counterpart in the reference, whose forwards recompute a series' whole context each time
  * (timestral/tornado/TimestralForward.java:187-642): for callers that keep a layer's keys and values while
- * patches arrive. The three calls below work on one layer's cache and may be captured into CUDA graphs. A call's
- * device arrays are read when its kernels run, on `stream`.
+ * patches arrive. The calls below work on one layer's cache, and those that launch may be captured into CUDA graphs. A
+ * call's device arrays are read when its kernels run, on `stream`.
  *
  * The pools (device memory, 16-byte aligned), contiguous, head_dim D 64 or 128, page_size a multiple of 16:
  *   bits 16: k, v [pages, kv_heads, page_size, D] in the call's precision (JC_BF16 or JC_FP16)
@@ -526,7 +526,8 @@ typedef struct jc_kv_cache {
  * whose start, length or page ids lie outside the call's bounds (pages: [0, cache pages)) is left out (an attention
  * row leaves out the page's keys), no memory outside the given arrays is touched, and the next jc_device_sync
  * returns JC_ERR_INVALID_ARG. Page ids past a sequence's length, and in pages that its tokens do not see, are not
- * read. No two sequences of an append may own one page that it writes.
+ * read. No two sequences of an append may own one page that it writes. Packed rows that no sequence's bounds take in are
+ * nobody's: their outputs are not written.
  */
 typedef struct jc_kv_step {
   int sequences;
@@ -569,8 +570,11 @@ jc_status jc_kv_append_device(int device, jc_precision precision, const jc_kv_ca
 /*
  * Attention of the step's new tokens over the cache (which holds them already): with index t, a token sees the keys
  * j <= t with j > t - window or j < sinks (window 0: every j <= t);
- *   out [tokens, heads, D] = sum_j softmax_j(scale * q.k_j) v_j, zeros for a token that sees no key.
- * Query head h reads kv head h / (heads / kv_heads). Statistics and sums are held in FP32. Values in slots that a
+ *   out [tokens, heads, D] = sum_j softmax_j(scale * q.k_j) v_j, zeros for a token that sees no key, NaN where a score is
+ *   NaN or every score is -inf.
+ * Query head h reads kv head h / (heads / kv_heads). Scores, statistics and sums are held in FP32; the probabilities are
+ * rounded to the precision (over a 4-bit cache: to FP16, and so are its queries, scaled by a power of two) for their product
+ * with v, whose sum is rounded once (FP16 saturating). Values in slots that a
  * token does not see never reach its output, whatever they are. `out` may be `q` itself; otherwise the two share no
  * element. `workspace` (16-byte aligned device memory, NULL
  * when jc_kv_attention_workspace says 0) holds partial results during the call; its contents do not matter.

@@ -31,8 +31,8 @@ namespace {
 
 constexpr int kWarps = 4;
 // CTAs that a call is split into where its rows alone are fewer: one wave of equal ones for one sequence (131,000 keys
-// over 4 bits: 52 us, 56 with two waves, 66 with four), many small ones for sequences of any lengths (48 of 5000 to 32,500
-// keys: 332 us, 367 with two waves).
+// over 4 bits, 64 dims in pages of 64: 52 us, 56 with two waves, 66 with four), many small ones for sequences of any lengths (48 of 5000 to 32,500
+// keys: 330 us, 367 with two waves).
 constexpr int kCtasOne = 148 * 4, kCtasMany = 148 * 16, kMaxSplits = kCtasMany;
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's running maximum moves only when a score passes it by this much (as a power of two): probabilities then
@@ -614,8 +614,9 @@ int subs_of(const KvAttnArgs& a) { return a.c.bits == 16 ? 1 : a.c.dim == 64 ? 4
 bool whole_steps(const KvAttnArgs& a) { return a.c.page_size % (16 * subs_of(a)) == 0; }
 
 // The most blocks that a tile reads, and how they are split: enough CTAs for every SM to hold some twice over, of at
-// least 128 keys a warp (a shorter loop is all latency), each split's partial result being a few rows of D floats
-// against chunk blocks of cache.
+// least 128 keys a warp (a shorter loop is all latency; a call a little above that pays a second launch: 3 sequences of 350
+// to 611 keys over 4 bits take 14 us, as a whole call of 16 bits 10), each split's partial result being a few rows of D
+// floats against chunk blocks of cache.
 SplitShape shape_of(const KvAttnArgs& a) {
   const long long group = a.heads / a.c.kv_heads, rpt = rows_per_tile(a);
   SplitShape sh{};
@@ -648,7 +649,7 @@ SplitShape shape_of(const KvAttnArgs& a) {
 
 template <typename T, int BITS, int D, bool WHOLE>
 void split(const KvAttnArgs& a, const SplitShape& sh, int rpt, dim3 grid, cudaStream_t s) {
-  // (pages of 16, 131,000 keys, 64 dims: 70 us by 32 keys, 91 by 64)
+  // (131,000 keys over 4 bits, 64 dims, pages of 16: 66 us by 32 keys, 85 by 64)
   constexpr int SUB = WHOLE ? kSubs<BITS, D> : 2;
   if (rpt == 8)
     kv_attention_split_kernel<T, BITS, D, 1, SUB, WHOLE><<<grid, 32 * kWarps, 0, s>>>(a, sh);

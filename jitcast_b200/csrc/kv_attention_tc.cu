@@ -10,8 +10,9 @@
 // a block of keys: pages may lie anywhere) and one MMA issuer. The two tiles alternate: while one tile's products run,
 // the other's exponentials do, and both read each K and V tile once from shared memory, which halves the bytes from L2.
 // What bounds it: at 64 dims the exponentials (128 · 128 a tile at 16 a clock and SM: 1024 clocks, against 512 for the
-// products), at 128 dims both alike; a step takes 1.5 to 1.9 times that, the latencies of the chain product → TMEM load
-// → exponentials → TMEM store → product that the other tile (or CTA) does not cover. Taking some exponentials on the FMA
+// products); at 128 dims the products' rate would take 1024 too, but S, both of whose operands come from shared memory, was
+// measured at 632 clocks a tile for 512 by rate. A step takes 1.5 to 1.9 times that, the latencies of the chain product →
+// TMEM load → exponentials → TMEM store → product that the other tile (or CTA) does not cover. Taking some exponentials on the FMA
 // units by a polynomial made it slower (issue slots), P in TMEM columns of its own too (one more handshake a step).
 //
 // S(j + 1) is issued after P·V(j) of its tile by the same thread, so when a softmax warp sees S(j + 1) ready, O holds

@@ -68,7 +68,7 @@ struct KvAttnArgs {
   int window;  // keys of the sliding window, the token's own included; 0: every key
   int sinks;   // first keys of a sequence that stay visible
   float scale;
-  float* workspace;  // partial results of split key ranges (KvPlan::workspace bytes)
+  float* workspace;  // partial results of split key ranges (kv_attention_workspace bytes)
   uint32_t* err;
 };
 

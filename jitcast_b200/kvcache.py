@@ -82,7 +82,8 @@ def _int32(t, name, dim, device=None):
 class Step:
     """The sequences of a call, shared by a model's layers: each one's cached ``length`` [n] (new tokens included)
     and its pages ``page_table`` [n, most pages], int32 on the GPU. ``start`` [n + 1] has the bounds of each
-    sequence's packed new tokens; without it every sequence has one. ``max_length`` and ``max_new`` bound the
+    sequence's packed new tokens (rows outside them are nobody's, their outputs are not written); without it every
+    sequence has one. ``max_length`` and ``max_new`` bound the
     lengths and the new tokens, and may be set anew as series grow. The tensors stay those of the start; what they hold
     may be rewritten between calls (they are read on the GPU)."""
 
